@@ -32,7 +32,7 @@ extern "C" {
 /* Changes whenever a struct layout or a signature of this header changes or an entry point is added; a caller built against another
  * value must not call into the library.  tc_struct_bytes lets a binding that restates the structs (ctypes)
  * verify its own layout: which = 0 tc_layer_weights, 1 tc_encoder_desc, 2 tc_layer_grads, 3 tc_encoder_grads. */
-#define TC_VERSION 131
+#define TC_VERSION 132
 
 /* status codes */
 #define TC_OK 0
@@ -686,6 +686,27 @@ int tc_crop_pad(const int32_t *in, int32_t *out, const int32_t *start, const int
 int tc_adamw_step(float *param, const float *grad, float *exp_avg, float *exp_avg_sq, long n, float lr,
                   float beta1, float beta2, float eps, float weight_decay, int step, float grad_scale,
                   void *stream);
+
+/* ---- embedding lookup with scaling, gradient by sorted tokens ---------------------------------
+ * The lookup of transcodon/model.py:178-206 for a table of any size:
+ *   out[m,:] = scale * table[tokens[m],:]   (multiplied in f32, rounded once to out_dtype)
+ * tokens: M ids of id_bytes (4 or 8) each.  Rows whose id is pad_idx (pad_idx < 0: none) are zeros, and so are
+ * rows whose id is outside [0, vocab); those also set *bad to 1 (bad may be NULL; it is never cleared).
+ * table [vocab,E] and out [M,E] dense, f32 or bf16 each; any E up to 65536.
+ */
+int tc_embedding_fwd(int table_dtype, int out_dtype, int id_bytes, const void *tokens, const void *table, void *out,
+                     long M, int E, long vocab, float scale, long pad_idx, int32_t *bad, void *stream);
+
+/*
+ * Its gradient: d_table[v,:] = (accumulate ? d_table[v,:] : 0) + scale * sum over m with tokens[m] == v of dy[m,:],
+ * f32, rows of pad_idx and of ids outside [0, vocab) left out (also where dy holds infinities or NaN there).  The
+ * positions are sorted by id inside the call and summed in a fixed order: the result is the same every time.
+ * dy [M,E] f32 or bf16, row stride ld_dy >= E; d_table [vocab,E] dense.  Without `accumulate` every row is written.
+ */
+size_t tc_embedding_bwd_workspace_bytes(long M, int E, long vocab);      /* 0: unsupported shape */
+int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, const void *dy, long ld_dy, float *d_table, long M,
+                     int E, long vocab, float scale, long pad_idx, int accumulate, void *workspace,
+                     size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

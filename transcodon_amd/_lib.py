@@ -11,7 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # TC_LIB_PATH points at another build of the same library (A/B timing of kernel variants)
 LIB_PATH = os.environ.get("TC_LIB_PATH") or os.path.join(_HERE, "csrc", "libtranscodon_hip.so")
 
-ABI_VERSION = 131          # TC_VERSION of include/transcodon_hip.h this binding restates
+ABI_VERSION = 132          # TC_VERSION of include/transcodon_hip.h this binding restates
 TC_F32, TC_BF16 = 0, 1
 EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESIDUAL, EPI_QKV_ROPE = 0, 1, 2, 3
 EPI_PLAIN_F32, EPI_BIAS_GELU_SAVE, EPI_DGELU = 4, 5, 6
@@ -147,6 +147,11 @@ _SIGNATURES = {
                               C.c_int, vp, C.c_int, vp]),
     "tc_crop_pad": (C.c_int, [vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp]),
     "tc_adamw_step": (C.c_int, [vp, vp, vp, vp, C.c_long] + [C.c_float] * 5 + [C.c_int, C.c_float, vp]),
+    "tc_embedding_fwd": (C.c_int, [C.c_int, C.c_int, C.c_int, vp, vp, vp, C.c_long, C.c_int, C.c_long, C.c_float, C.c_long,
+                                   vp, vp]),
+    "tc_embedding_bwd_workspace_bytes": (C.c_size_t, [C.c_long, C.c_int, C.c_long]),
+    "tc_embedding_bwd": (C.c_int, [C.c_int, C.c_int, vp, vp, C.c_long, vp, C.c_long, C.c_int, C.c_long, C.c_float, C.c_long,
+                                   C.c_int, vp, C.c_size_t, vp]),
     "tc_prof_enable": (C.c_int, [C.c_int]),
     "tc_prof_reset": (C.c_int, []),
     "tc_prof_collect": (C.c_int, [C.c_int, C.POINTER(C.c_int64), C.POINTER(C.c_double),

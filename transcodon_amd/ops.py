@@ -322,3 +322,103 @@ def colsum(x, want_bf16_copy=False, out=None):
     copy = torch.empty(M, N, dtype=torch.bfloat16, device=x.device) if want_bf16_copy else None
     check(_lib.load().tc_colsum(_dt(x), _p(x), x.stride(0), _p(copy), N, _p(out), M, N, _stream()), "tc_colsum")
     return (out, copy) if want_bf16_copy else out
+
+
+# ---- operators of a training block ---------------------------------------------------------------
+def _same_device(*tensors):
+    """The common device of GPU tensors (None entries skipped); raises otherwise."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.HipLibraryError("transcodon_amd kernels need tensors on the GPU (no CPU fallback)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return dev
+
+
+def _call(name, dev, *args):
+    """One library call on ``dev``'s current stream, also where another device is the current one."""
+    fn = getattr(_lib.load(), name)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    check(rc, name)
+
+
+def _rows(t, name):
+    """Row stride of a 2-d tensor whose columns are neighbours in memory."""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        raise ValueError(f"{name} must be 2-d with unit column stride and rows that do not overlap")
+    return max(t.stride(0), t.shape[1])
+
+
+def _dense(t, name, shape=None, dtype=None):
+    """Checks a dense operand: its shape and element type where they are given."""
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} has type {t.dtype}, expected {dtype}")
+
+
+def _id_bytes(tokens):
+    if tokens.dtype == torch.int32:
+        return 4
+    if tokens.dtype == torch.int64:
+        return 8
+    raise TypeError(f"token ids must be int32 or int64, got {tokens.dtype}")
+
+
+def embedding(tokens, table, scale=1.0, pad_idx=None, out_dtype=None, bad=None):
+    """scale * table[tokens] -> [tokens.numel(), E] in ``out_dtype`` (default: the table's type), zeros for ``pad_idx`` and for
+    ids outside the table; the latter also set ``bad`` (int32 [1], optional, never cleared here).  tc_embedding_fwd; the lookup
+    of model.py:178-206 for a table of any size."""
+    dev = _same_device(tokens, table, bad)
+    idb = _id_bytes(tokens)
+    _dense(tokens, "tokens")
+    if table.dim() != 2:
+        raise ValueError("table must be [vocab, E]")
+    _dense(table, "table")
+    if bad is not None:
+        _dense(bad, "bad", (1,), torch.int32)
+    V, E = table.shape
+    M = tokens.numel()
+    out = torch.empty(M, E, dtype=out_dtype or table.dtype, device=dev)
+    dts = _dt(table), _dt(out)
+    if M and E:
+        _call("tc_embedding_fwd", dev, *dts, idb, tokens.data_ptr(), table.data_ptr(), out.data_ptr(), M, E, V, scale,
+              -1 if pad_idx is None else pad_idx, _p(bad))
+    return out
+
+
+def embedding_bwd(tokens, dy, vocab, scale=1.0, pad_idx=None, out=None):
+    """Gradient of :func:`embedding` with respect to its table: f32 [vocab, E], summed by sorted tokens in a fixed order
+    (added to ``out`` when given).  dy [tokens.numel(), E] f32 or bf16, rows may be strided.  tc_embedding_bwd."""
+    dev = _same_device(tokens, dy, out)
+    idb = _id_bytes(tokens)
+    _dense(tokens, "tokens")
+    ld = _rows(dy, "dy")
+    M, E = dy.shape
+    if tokens.numel() != M:
+        raise ValueError(f"{tokens.numel()} tokens but {M} rows of dy")
+    accumulate = out is not None
+    if accumulate:
+        _dense(out, "out", (vocab, E), torch.float32)
+    elif M == 0 or E == 0:
+        return torch.zeros(vocab, E, dtype=torch.float32, device=dev)
+    else:
+        out = torch.empty(vocab, E, dtype=torch.float32, device=dev)
+    dt = _dt(dy)
+    if M and E:
+        need = _lib.load().tc_embedding_bwd_workspace_bytes(M, E, vocab)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        _call("tc_embedding_bwd", dev, dt, idb, tokens.data_ptr(), dy.data_ptr(), ld, out.data_ptr(), M, E, vocab, scale,
+              -1 if pad_idx is None else pad_idx, int(accumulate), ws.data_ptr(), need)
+    return out
