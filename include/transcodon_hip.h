@@ -708,6 +708,37 @@ int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, const void 
                      int E, long vocab, float scale, long pad_idx, int accumulate, void *workspace,
                      size_t workspace_bytes, void *stream);
 
+/* ---- norms before and after a block, with gate and residual scale ---------------------------------
+ * One pass over the rows:
+ *   n     = norm(y; post_eps) * post_gamma + post_beta
+ *   x_out = res_scale * x + gate o n
+ *   h     = norm(x_out; pre_eps) * pre_gamma + pre_beta
+ * norm(t) = (t - mean(t)) / sqrt(var(t) + eps), or with rms != 0 t / sqrt(mean(t^2) + eps).
+ * y, h: dtype (f32 or bf16); x, x_out and the vectors: f32; gate: f32, or bf16 with bf16 rows, [G,E] where row g is
+ * for rows g M/G .. (g+1) M/G - 1 (G = 1: one for all, G = M: one for each; gate NULL and G = 0: none).  The betas may be NULL;
+ * pre_gamma, pre_beta and h NULL leave the second norm out.  y and x may have row strides ldy, ldx >= E; x_out may be x.
+ * stats (optional) [M,4] f32: mean and 1/deviation of y, then of x_out (0, 0 without the second norm).  E <= 8192.
+ */
+int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, const float *x, long ldx, const float *post_gamma,
+                               const float *post_beta, int gate_dtype, const void *gate, int G, float res_scale,
+                               const float *pre_gamma, const float *pre_beta, float *x_out, void *h, float *stats,
+                               long M, int E, int rms, float post_eps, float pre_eps, void *stream);
+
+/*
+ * Its gradient.  dh (dtype; NULL without the second norm) and dx_out (f32; may be NULL) are the gradients of h and
+ * x_out, y, x_out and stats those of the forward pass.  Writes dy (dtype) and dx (f32; may be dx_out) dense, and the f32
+ * gradients of the vectors and of the gate [G,E] (d_gate goes with gate; the others may be NULL).  accumulate: bits 0 .. 4 add to
+ * d_post_gamma, d_post_beta, d_pre_gamma, d_pre_beta, d_gate instead of overwriting them.  Column sums have a fixed order:
+ * the result is the same every time.
+ */
+size_t tc_gated_residual_norm_bwd_workspace_bytes(long M, int E, int G);     /* 0: unsupported shape */
+int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh, const float *dx_out, long ld_dxo, const void *y, long ldy,
+                               const float *x_out, long ldx, const float *stats, const float *post_gamma,
+                               const float *post_beta, int gate_dtype, const void *gate, int G, float res_scale,
+                               const float *pre_gamma, void *dy, float *dx, float *d_post_gamma, float *d_post_beta,
+                               float *d_gate, float *d_pre_gamma, float *d_pre_beta, int accumulate, long M, int E, int rms,
+                               void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -152,6 +152,12 @@ _SIGNATURES = {
     "tc_embedding_bwd_workspace_bytes": (C.c_size_t, [C.c_long, C.c_int, C.c_long]),
     "tc_embedding_bwd": (C.c_int, [C.c_int, C.c_int, vp, vp, C.c_long, vp, C.c_long, C.c_int, C.c_long, C.c_float, C.c_long,
                                    C.c_int, vp, C.c_size_t, vp]),
+    "tc_gated_residual_norm_fwd": (C.c_int, [C.c_int, vp, C.c_long, vp, C.c_long, vp, vp, C.c_int, vp, C.c_int, C.c_float, vp,
+                                             vp, vp, vp, vp, C.c_long, C.c_int, C.c_int, C.c_float, C.c_float, vp]),
+    "tc_gated_residual_norm_bwd_workspace_bytes": (C.c_size_t, [C.c_long, C.c_int, C.c_int]),
+    "tc_gated_residual_norm_bwd": (C.c_int, [C.c_int, vp, C.c_long, vp, C.c_long, vp, C.c_long, vp, C.c_long, vp, vp, vp,
+                                             C.c_int, vp, C.c_int, C.c_float, vp, vp, vp, vp, vp, vp, vp, vp, C.c_int,
+                                             C.c_long, C.c_int, C.c_int, vp, C.c_size_t, vp]),
     "tc_prof_enable": (C.c_int, [C.c_int]),
     "tc_prof_reset": (C.c_int, []),
     "tc_prof_collect": (C.c_int, [C.c_int, C.POINTER(C.c_int64), C.POINTER(C.c_double),

@@ -1,0 +1,524 @@
+// The end of one residual block and the start of the next in one pass:
+//
+//   n     = norm_post(y) * g1 + b1                norm after the block (y: the block's output)
+//   x_out = res_scale * x + gate o n              gate: a row of [G,E] for M / G consecutive rows, or none
+//   h     = norm_pre(x_out) * g2 + b2             norm before the next block (left out where g2 is null)
+//
+// and its backward pass.  norm(t) = (t - mean) * rstd, or t * rstd for root-mean-square norms (mean = 0).  The residual
+// stream and all arithmetic are f32; y, h and their gradients are f32 or bf16.
+//
+// A team of W waves owns a row at a time and keeps it in registers (W = 1 up to 1024 columns), so every operand is
+// read from memory once; deviations are summed after the mean is known.  The backward pass gives each team a run of
+// neighbouring rows and keeps the column sums (gradients of the norms' vectors and of the gate) in registers; teams of
+// a workgroup are added in LDS, workgroups by a second kernel, always in the same order.
+#include "row_io.h"
+
+namespace {
+
+template <int W>
+struct Team {                                // W waves that work on one row
+    float (*lds)[2][W];                      // [turn][value][wave]
+    int wave, turn = 0;
+    // sums of a and b over the team's lanes, on every lane
+    __device__ __forceinline__ void sum2(float &a, float &b) {
+        a = tc_wave_sum(a);
+        b = tc_wave_sum(b);
+        if constexpr (W > 1) {
+            // two buffers in turn: a wave writes one only after the barrier that follows every read of it
+            if ((threadIdx.x & 63) == 0) { lds[turn][0][wave] = a; lds[turn][1][wave] = b; }
+            __syncthreads();
+            a = b = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) { a += lds[turn][0][w]; b += lds[turn][1][w]; }
+            turn ^= 1;
+        }
+    }
+    __device__ __forceinline__ float sum(float a) {
+        float unused = 0.f;
+        sum2(a, unused);
+        return a;
+    }
+};
+
+// mean and 1 / sqrt(variance + eps) of a row held as v[NC][VEC]
+template <int W, int NC, int VEC>
+__device__ __forceinline__ void row_stats(Team<W> &team, const float (&v)[NC][VEC], const bool (&in)[NC], int E, int rms, float eps,
+                                          float &mean, float &rstd) {
+    mean = 0.f;
+    if (!rms) {
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s += v[c][j];          // zero past the end of the row
+        mean = team.sum(s) / (float)E;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+        if (in[c]) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float d = v[c][j] - mean;
+                q += d * d;
+            }
+        }
+    rstd = rsqrtf(team.sum(q) / (float)E + eps);
+}
+
+struct NormParams {
+    const void *y, *gate;
+    const float *x, *g1, *b1, *g2, *b2;
+    float *x_out, *stats;
+    void *h;
+    // backward
+    const void *dh;
+    const float *dx_out;
+    void *dy;
+    float *dx, *d_gate, *ws;
+    float *d_vec[4];                         // gradients of g1, b1, g2, b2 (null: not wanted)
+    int accumulate;                          // bit v: add to d_vec[v]; bit 4: add to d_gate
+    long ldy, ldx, ld_dh, ld_dxo;
+    int M, E, rms;
+    int rows_per_gate;                       // M / G (M without a gate)
+    float res_scale, eps1, eps2;
+    // backward: team t owns rows [t * rows_per_team, ...) of whole gate groups, or a part of one group
+    int teams, rows_per_team, teams_per_group;
+};
+
+template <typename T, typename TG, int VEC, int W, int NC>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_kernel(const NormParams p) {
+    __shared__ float red[2][2][W];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Team<W> team{red, W == 1 ? 0 : wave};
+    constexpr int kTeams = W == 1 ? 4 : 1;
+    const int col0 = ((W == 1 ? 0 : wave) * 64 + lane) * VEC;
+    bool in[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) in[c] = col0 + c * 64 * W * VEC < p.E;
+    for (long row = (long)blockIdx.x * kTeams + (W == 1 ? wave : 0); row < p.M; row += (long)gridDim.x * kTeams) {
+        float yv[NC][VEC], xv[NC][VEC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = col0 + c * 64 * W * VEC;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) yv[c][j] = xv[c][j] = 0.f;
+            if (in[c]) {
+                tc_load_row<T, VEC>(static_cast<const T *>(p.y) + row * p.ldy + col, yv[c]);
+                tc_load_row<float, VEC>(p.x + row * p.ldx + col, xv[c]);
+            }
+        }
+        float mean1, rstd1;
+        row_stats<W, NC, VEC>(team, yv, in, p.E, p.rms, p.eps1, mean1, rstd1);
+        const long gate_row = (row / p.rows_per_gate) * p.E;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = col0 + c * 64 * W * VEC;
+            if (!in[c]) continue;
+            float g[VEC], b[VEC], gt[VEC];
+            tc_load_row<float, VEC>(p.g1 + col, g);
+            if (p.b1) tc_load_row<float, VEC>(p.b1 + col, b);
+            if (p.gate) tc_load_row<TG, VEC>(static_cast<const TG *>(p.gate) + gate_row + col, gt);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                float n = (yv[c][j] - mean1) * rstd1 * g[j];
+                if (p.b1) n += b[j];
+                if (p.gate) n *= gt[j];
+                xv[c][j] = p.res_scale * xv[c][j] + n;
+            }
+            tc_store_row<float, VEC>(p.x_out + row * p.E + col, xv[c]);
+        }
+        float mean2 = 0.f, rstd2 = 0.f;
+        if (p.g2) {
+            row_stats<W, NC, VEC>(team, xv, in, p.E, p.rms, p.eps2, mean2, rstd2);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int col = col0 + c * 64 * W * VEC;
+                if (!in[c]) continue;
+                float g[VEC], b[VEC];
+                tc_load_row<float, VEC>(p.g2 + col, g);
+                if (p.b2) tc_load_row<float, VEC>(p.b2 + col, b);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    xv[c][j] = (xv[c][j] - mean2) * rstd2 * g[j];
+                    if (p.b2) xv[c][j] += b[j];
+                }
+                tc_store_row<T, VEC>(static_cast<T *>(p.h) + row * p.E + col, xv[c]);
+            }
+        }
+        if (p.stats && col0 == 0) *reinterpret_cast<f32x4 *>(p.stats + row * 4) = f32x4{mean1, rstd1, mean2, rstd2};
+    }
+}
+
+// Gradient.  With D = d(loss)/d(x_out) in full:
+//   x^ = (x_out - mean2) rstd2    D = dx_out + rstd2 (p - mean(p) - x^ mean(p x^)),  p = dh o g2
+//   y^ = (y - mean1) rstd1        dn = D o gate     dy = rstd1 (q - mean(q) - y^ mean(q y^)),  q = dn o g1
+//   dx = res_scale D    d_gate = sum D o n    d_g1 = sum dn o y^   d_b1 = sum dn   d_g2 = sum dh o x^   d_b2 = sum dh
+// (root-mean-square norms: without the mean(p), mean(q) terms).
+template <typename T, typename TG, int VEC, int W, int NC>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(const NormParams p) {
+    extern __shared__ float sums[];          // [4][E] of the workgroup (W == 1)
+    __shared__ float red[2][2][W];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Team<W> team{red, W == 1 ? 0 : wave};
+    constexpr int kTeams = W == 1 ? 4 : 1;   // teams of a workgroup
+    const int t = blockIdx.x * kTeams + (W == 1 ? wave : 0);
+    const int col0 = ((W == 1 ? 0 : wave) * 64 + lane) * VEC;
+    bool in[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) in[c] = col0 + c * 64 * W * VEC < p.E;
+    float acc[4][NC][VEC], dgt[NC][VEC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            acc[0][c][j] = acc[1][c][j] = acc[2][c][j] = acc[3][c][j] = 0.f;
+            dgt[c][j] = 0.f;
+        }
+    // rows of this team
+    long begin, end;
+    if (p.teams_per_group > 0) {
+        const int g = t / p.teams_per_group, part = t - g * p.teams_per_group;
+        begin = (long)g * p.rows_per_gate + (long)part * p.rows_per_team;
+        end = min((long)(g + 1) * p.rows_per_gate, begin + p.rows_per_team);
+    } else {
+        begin = (long)t * p.rows_per_team;
+        end = min((long)p.M, begin + p.rows_per_team);
+    }
+    if (t >= p.teams) begin = end = 0;
+    const float inv_e = 1.0f / (float)p.E;
+    for (long row = begin; row < end; ++row) {
+        float yv[NC][VEC], xv[NC][VEC], dh[NC][VEC], d[NC][VEC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = col0 + c * 64 * W * VEC;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) yv[c][j] = xv[c][j] = dh[c][j] = d[c][j] = 0.f;
+            if (in[c]) {
+                tc_load_row<T, VEC>(static_cast<const T *>(p.y) + row * p.ldy + col, yv[c]);
+                if (p.g2) {
+                    tc_load_row<float, VEC>(p.x + row * p.ldx + col, xv[c]);
+                    tc_load_row<T, VEC>(static_cast<const T *>(p.dh) + row * p.ld_dh + col, dh[c]);
+                }
+                if (p.dx_out) tc_load_row<float, VEC>(p.dx_out + row * p.ld_dxo + col, d[c]);
+            }
+        }
+        const f32x4 st = *reinterpret_cast<const f32x4 *>(p.stats + row * 4);
+        if (p.g2) {
+            float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int col = col0 + c * 64 * W * VEC;
+                if (!in[c]) continue;
+                float g[VEC];
+                tc_load_row<float, VEC>(p.g2 + col, g);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float xh = (xv[c][j] - st[2]) * st[3];
+                    acc[2][c][j] += dh[c][j] * xh;
+                    acc[3][c][j] += dh[c][j];
+                    const float q = dh[c][j] * g[j];
+                    s1 += q;
+                    s2 += q * xh;
+                    xv[c][j] = xh;
+                    dh[c][j] = q;
+                }
+            }
+            team.sum2(s1, s2);
+            const float m1 = p.rms ? 0.f : s1 * inv_e, m2 = s2 * inv_e;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) d[c][j] += st[3] * (dh[c][j] - m1 - xv[c][j] * m2);
+        }
+        const long gate_row = (row / p.rows_per_gate) * p.E;
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = col0 + c * 64 * W * VEC;
+            if (!in[c]) continue;
+            float g[VEC], b[VEC], gt[VEC], o[VEC];
+            tc_load_row<float, VEC>(p.g1 + col, g);
+            if (p.gate) tc_load_row<TG, VEC>(static_cast<const TG *>(p.gate) + gate_row + col, gt);
+            if (p.gate && p.b1) tc_load_row<float, VEC>(p.b1 + col, b);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float yh = (yv[c][j] - st[0]) * st[1];
+                float dn = d[c][j];
+                if (p.gate) {
+                    float n = yh * g[j];
+                    if (p.b1) n += b[j];
+                    dgt[c][j] += dn * n;
+                    dn *= gt[j];
+                }
+                acc[0][c][j] += dn * yh;
+                acc[1][c][j] += dn;
+                const float q = dn * g[j];
+                s1 += q;
+                s2 += q * yh;
+                o[j] = p.res_scale * d[c][j];
+                yv[c][j] = yh;
+                d[c][j] = q;
+            }
+            tc_store_row<float, VEC>(p.dx + row * p.E + col, o);
+        }
+        team.sum2(s1, s2);
+        const float m1 = p.rms ? 0.f : s1 * inv_e, m2 = s2 * inv_e;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = col0 + c * 64 * W * VEC;
+            if (!in[c]) continue;
+            float o[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) o[j] = st[1] * (d[c][j] - m1 - yv[c][j] * m2);
+            tc_store_row<T, VEC>(static_cast<T *>(p.dy) + row * p.E + col, o);
+        }
+        // the team's last row of a gate group: the group's gradient, or this team's part of it
+        if (p.gate && p.teams_per_group == 0 && (row + 1) % p.rows_per_gate == 0) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int col = col0 + c * 64 * W * VEC;
+                if (!in[c]) continue;
+                float *to = p.d_gate + gate_row + col;
+                if (p.accumulate & 16) {
+                    float old[VEC];
+                    tc_load_row<float, VEC>(to, old);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) dgt[c][j] += old[j];
+                }
+                tc_store_row<float, VEC>(to, dgt[c]);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) dgt[c][j] = 0.f;
+            }
+        }
+    }
+    // workspace: [workgroups][4][E] vectors, then [teams][E] gate parts
+    if (p.gate && p.teams_per_group > 0 && t < p.teams) {
+        float *to = p.ws + (long)gridDim.x * 4 * p.E + (long)t * p.E;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = col0 + c * 64 * W * VEC;
+            if (in[c])
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) to[col + j] = dgt[c][j];
+        }
+    }
+    float *to = p.ws + (long)blockIdx.x * 4 * p.E;
+    if constexpr (W == 1) {
+        for (int w = 0; w < kTeams; ++w) {
+            if (wave == w) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        const int col = col0 + c * 64 * VEC;
+                        if (in[c])
+#pragma unroll
+                            for (int j = 0; j < VEC; ++j) sums[v * p.E + col + j] = w == 0 ? acc[v][c][j] : sums[v * p.E + col + j] + acc[v][c][j];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < 4 * p.E; i += 256) to[i] = sums[i];
+    } else {
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int col = col0 + c * 64 * W * VEC;
+                if (in[c])
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) to[(long)v * p.E + col + j] = acc[v][c][j];
+            }
+    }
+}
+
+// Column sums of the parts that the workgroups (v < 4: a vector's gradient) or the teams of a gate group (v - 4: the
+// group) left: 64 columns per workgroup, 16 row lanes, added in a fixed order.
+__global__ __launch_bounds__(1024) void gated_norm_join_kernel(const NormParams p, int workgroups, int groups) {
+    __shared__ float red[16][64];
+    const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
+    const int col = blockIdx.x * 64 + c;
+    for (int v = blockIdx.y; v < 4 + groups; v += gridDim.y) {
+        const bool vec = v < 4;
+        const int g = v - 4, n = vec ? workgroups : p.teams_per_group;
+        float *out = vec ? p.d_vec[v] : p.d_gate + (long)g * p.E;
+        const float *src = vec ? p.ws + (long)v * p.E : p.ws + (long)workgroups * 4 * p.E + (long)g * n * p.E;
+        const long ld = vec ? 4L * p.E : p.E;
+        if (!out) continue;
+        float s = 0.f;
+        if (col < p.E)
+#pragma unroll 4
+            for (int i = r; i < n; i += 16) s += src[i * ld + col];
+        red[r][c] = s;
+        __syncthreads();
+        if (r == 0 && col < p.E) {
+            for (int i = 1; i < 16; ++i) s += red[i][c];
+            out[col] = (p.accumulate >> (vec ? v : 4)) & 1 ? out[col] + s : s;
+        }
+        __syncthreads();
+    }
+}
+
+// Waves per row and values per lane: one wave up to 1024 columns, four up to 4096, eight up to 8192.
+int waves_per_row(int E) { return E <= 1024 ? 1 : E <= 4096 ? 4 : 8; }
+
+struct BwdPlan {
+    int teams, rows_per_team, teams_per_group, workgroups;
+    size_t bytes;
+};
+BwdPlan bwd_plan(int M, int E, int G) {
+    BwdPlan w{};
+    const int W = waves_per_row(E), per_wg = W == 1 ? 4 : 1;
+    const int want = 2048 / W * (W == 1 ? 1 : 2);
+    const int rows = (M + want - 1) / want;
+    const int group = G > 0 ? M / G : 0;
+    if (G == 0 || group <= rows) {
+        w.rows_per_team = G == 0 ? rows : rows / group * group;
+        w.teams = (M + w.rows_per_team - 1) / w.rows_per_team;
+    } else {
+        w.teams_per_group = (group + rows - 1) / rows;
+        w.rows_per_team = (group + w.teams_per_group - 1) / w.teams_per_group;
+        w.teams = G * w.teams_per_group;
+    }
+    w.workgroups = (w.teams + per_wg - 1) / per_wg;
+    w.bytes = ((size_t)w.workgroups * 4 + (w.teams_per_group > 0 ? w.teams : 0)) * E * sizeof(float);
+    return w;
+}
+
+int check_common(const char *who, int dtype, int gate_dtype, const void *gate, long M, int E, int G) {
+    TC_REQUIRE(dtype == TC_F32 || dtype == TC_BF16, "%s: bad dtype %d", who, dtype);
+    TC_REQUIRE(M > 0 && M <= 0x7fffffffL && E > 0 && E <= 8192, "%s: bad shape M=%ld E=%d (E <= 8192)", who, M, E);
+    TC_REQUIRE((gate != nullptr) == (G > 0), "%s: a gate and its %d rows go together", who, G);
+    TC_REQUIRE(G >= 0 && (G == 0 || M % G == 0), "%s: %d gate rows do not divide %ld rows", who, G, M);
+    TC_REQUIRE(gate_dtype == TC_F32 || (gate_dtype == TC_BF16 && dtype == TC_BF16), "%s: bad gate type %d", who, gate_dtype);
+    TC_REQUIRE((uintptr_t)gate % (gate_dtype == TC_BF16 ? 2 : 4) == 0, "%s: misaligned gate", who);
+    return TC_OK;
+}
+
+}  // namespace
+
+#define TC_GN_NC(K, T, TG, W)                                                                   \
+    do {                                                                                        \
+        if (!vec) TC_GN(K, T, TG, 1, W, 16);                                                    \
+        else if (E <= 64 * 4 * W) TC_GN(K, T, TG, 4, W, 1);                                     \
+        else if (E <= 64 * 8 * W) TC_GN(K, T, TG, 4, W, 2);                                     \
+        else if (E <= 64 * 12 * W) TC_GN(K, T, TG, 4, W, 3);                                    \
+        else TC_GN(K, T, TG, 4, W, 4);                                                          \
+    } while (0)
+#define TC_GN_W(K, T, TG)                                                                       \
+    do {                                                                                        \
+        if (W == 1) TC_GN_NC(K, T, TG, 1);                                                      \
+        else if (W == 4) TC_GN_NC(K, T, TG, 4);                                                 \
+        else TC_GN_NC(K, T, TG, 8);                                                             \
+    } while (0)
+#define TC_GN_T(K)                                                                              \
+    do {                                                                                        \
+        if (dtype == TC_F32) TC_GN_W(K, float, float);                                          \
+        else if (gate_dtype == TC_F32) TC_GN_W(K, uint16_t, float);                             \
+        else TC_GN_W(K, uint16_t, uint16_t);                                                    \
+    } while (0)
+
+extern "C" int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, const float *x, long ldx, const float *post_gamma,
+                                          const float *post_beta, int gate_dtype, const void *gate, int G, float res_scale,
+                                          const float *pre_gamma, const float *pre_beta, float *x_out, void *h, float *stats,
+                                          long M, int E, int rms, float post_eps, float pre_eps, void *stream) {
+    const int rc = check_common("tc_gated_residual_norm_fwd", dtype, gate_dtype, gate, M, E, G);
+    if (rc != TC_OK) return rc;
+    TC_REQUIRE(y && x && post_gamma && x_out, "tc_gated_residual_norm_fwd: null operand");
+    TC_REQUIRE((pre_gamma != nullptr) == (h != nullptr) && (pre_gamma || !pre_beta),
+               "tc_gated_residual_norm_fwd: the second norm's vectors and h go together");
+    TC_REQUIRE(ldy >= E && ldx >= E, "tc_gated_residual_norm_fwd: row stride below E");
+    const int esz = dtype == TC_BF16 ? 2 : 4;
+    TC_REQUIRE((uintptr_t)y % esz == 0 && (uintptr_t)h % esz == 0 && tc_aligned16(stats) &&
+                   ((uintptr_t)x | (uintptr_t)x_out | (uintptr_t)post_gamma | (uintptr_t)post_beta | (uintptr_t)pre_gamma |
+                    (uintptr_t)pre_beta) % 4 == 0,
+               "tc_gated_residual_norm_fwd: misaligned operand (stats: 16 bytes)");
+    NormParams p{};
+    p.y = y; p.x = x; p.gate = gate;
+    p.g1 = post_gamma; p.b1 = post_beta; p.g2 = pre_gamma; p.b2 = pre_beta;
+    p.x_out = x_out; p.h = h; p.stats = stats;
+    p.ldy = ldy; p.ldx = ldx;
+    p.M = (int)M; p.E = E; p.rms = rms;
+    p.rows_per_gate = G > 0 ? (int)(M / G) : (int)M;
+    p.res_scale = res_scale; p.eps1 = post_eps; p.eps2 = pre_eps;
+    const int g_esz = gate_dtype == TC_BF16 ? 2 : 4;
+    const bool vec = tc_rows_aligned(y, ldy, esz, 4) && tc_rows_aligned(x, ldx, 4, 4) && tc_rows_aligned(gate, E, g_esz, 4) &&
+                     tc_rows_aligned(h, E, esz, 4) && tc_aligned16(x_out) && tc_aligned16(post_gamma) && tc_aligned16(post_beta) &&
+                     tc_aligned16(pre_gamma) && tc_aligned16(pre_beta);
+    const int W = waves_per_row(E), per_wg = W == 1 ? 4 : 1;
+    long blocks = (M + per_wg - 1) / per_wg;
+    const long most = 1L << 22;                    // a launch holds fewer than 2^32 threads; rows are walked with the grid's stride
+    if (blocks > most) blocks = most;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    TcProfScope prof(TC_PROF_LAYERNORM, s, (double)M * E * (2 * esz + 8));
+#define TC_GN(K, T, TG, V, WW, N) TC_LAUNCH((K<T, TG, V, WW, N>), dim3((unsigned)blocks), dim3(WW == 1 ? 256 : 64 * WW), 0, s, p)
+    TC_GN_T(gated_norm_kernel);
+#undef TC_GN
+    TC_CHECK_LAUNCH("tc_gated_residual_norm_fwd");
+    return TC_OK;
+}
+
+extern "C" size_t tc_gated_residual_norm_bwd_workspace_bytes(long M, int E, int G) {
+    if (M <= 0 || M > 0x7fffffffL || E <= 0 || E > 8192 || G < 0 || (G > 0 && M % G != 0)) return 0;
+    return bwd_plan((int)M, E, G).bytes;
+}
+
+extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh, const float *dx_out, long ld_dxo, const void *y,
+                                          long ldy, const float *x_out, long ldx, const float *stats, const float *post_gamma,
+                                          const float *post_beta, int gate_dtype, const void *gate, int G, float res_scale,
+                                          const float *pre_gamma, void *dy, float *dx, float *d_post_gamma,
+                                          float *d_post_beta, float *d_gate, float *d_pre_gamma, float *d_pre_beta,
+                                          int accumulate, long M, int E, int rms, void *workspace, size_t workspace_bytes,
+                                          void *stream) {
+    const int rc = check_common("tc_gated_residual_norm_bwd", dtype, gate_dtype, gate, M, E, G);
+    if (rc != TC_OK) return rc;
+    TC_REQUIRE(y && x_out && stats && post_gamma && dy && dx && workspace, "tc_gated_residual_norm_bwd: null operand");
+    TC_REQUIRE((pre_gamma != nullptr) == (dh != nullptr) && (pre_gamma || (!d_pre_gamma && !d_pre_beta)),
+               "tc_gated_residual_norm_bwd: the second norm's vector, its gradients and dh go together");
+    TC_REQUIRE(dh || dx_out, "tc_gated_residual_norm_bwd: neither dh nor dx_out");
+    TC_REQUIRE((gate != nullptr) == (d_gate != nullptr), "tc_gated_residual_norm_bwd: a gate and its gradient go together");
+    TC_REQUIRE(ldy >= E && ldx >= E && (!dh || ld_dh >= E) && (!dx_out || ld_dxo >= E),
+               "tc_gated_residual_norm_bwd: row stride below E");
+    const int esz = dtype == TC_BF16 ? 2 : 4;
+    TC_REQUIRE(((uintptr_t)y | (uintptr_t)dh | (uintptr_t)dy) % esz == 0 && tc_aligned16(stats) && tc_aligned16(workspace) &&
+                   ((uintptr_t)x_out | (uintptr_t)dx_out | (uintptr_t)dx | (uintptr_t)post_gamma | (uintptr_t)post_beta |
+                    (uintptr_t)pre_gamma | (uintptr_t)d_post_gamma | (uintptr_t)d_post_beta | (uintptr_t)d_gate |
+                    (uintptr_t)d_pre_gamma | (uintptr_t)d_pre_beta) % 4 == 0,
+               "tc_gated_residual_norm_bwd: misaligned operand (stats and workspace: 16 bytes)");
+    const BwdPlan w = bwd_plan((int)M, E, G);
+    if (workspace_bytes < w.bytes) {
+        tc_set_error("tc_gated_residual_norm_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, w.bytes);
+        return TC_ENOSPC;
+    }
+    NormParams p{};
+    p.y = y; p.x = x_out; p.gate = gate; p.dh = dh; p.dx_out = dx_out;
+    p.stats = const_cast<float *>(stats);
+    p.g1 = post_gamma; p.b1 = post_beta; p.g2 = pre_gamma;
+    p.dy = dy; p.dx = dx; p.d_gate = d_gate;
+    p.ws = static_cast<float *>(workspace);
+    p.d_vec[0] = d_post_gamma; p.d_vec[1] = d_post_beta; p.d_vec[2] = d_pre_gamma; p.d_vec[3] = d_pre_beta;
+    p.accumulate = accumulate;
+    p.ldy = ldy; p.ldx = ldx; p.ld_dh = ld_dh; p.ld_dxo = ld_dxo;
+    p.M = (int)M; p.E = E; p.rms = rms;
+    p.rows_per_gate = G > 0 ? (int)(M / G) : (int)M;
+    p.res_scale = res_scale;
+    p.teams = w.teams; p.rows_per_team = w.rows_per_team; p.teams_per_group = w.teams_per_group;
+    const int g_esz = gate_dtype == TC_BF16 ? 2 : 4;
+    const bool vec = tc_rows_aligned(y, ldy, esz, 4) && tc_rows_aligned(x_out, ldx, 4, 4) && tc_rows_aligned(gate, E, g_esz, 4) &&
+                     (!dh || tc_rows_aligned(dh, ld_dh, esz, 4)) && (!dx_out || tc_rows_aligned(dx_out, ld_dxo, 4, 4)) &&
+                     tc_rows_aligned(dy, E, esz, 4) && tc_aligned16(dx) && tc_aligned16(d_gate) && tc_aligned16(post_gamma) &&
+                     tc_aligned16(post_beta) && tc_aligned16(pre_gamma);
+    const int W = waves_per_row(E);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    TcProfScope prof(TC_PROF_LAYERNORM, s, (double)M * E * (3 * esz + 12));
+#define TC_GN(K, T, TG, V, WW, N)                                                                                         \
+    TC_LAUNCH((K<T, TG, V, WW, N>), dim3((unsigned)w.workgroups), dim3(WW == 1 ? 256 : 64 * WW), WW == 1 ? 16 * (size_t)E : 0, s, p)
+    TC_GN_T(gated_norm_bwd_kernel);
+#undef TC_GN
+    const int groups = w.teams_per_group > 0 ? G : 0;
+    const int tall = 4 + groups < 1024 ? 4 + groups : 1024;
+    TC_LAUNCH(gated_norm_join_kernel, dim3((E + 63) / 64, tall), dim3(1024), 0, s, p, w.workgroups, groups);
+    TC_CHECK_LAUNCH("tc_gated_residual_norm_bwd");
+    return TC_OK;
+}

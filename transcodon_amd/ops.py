@@ -422,3 +422,101 @@ def embedding_bwd(tokens, dy, vocab, scale=1.0, pad_idx=None, out=None):
         _call("tc_embedding_bwd", dev, dt, idb, tokens.data_ptr(), dy.data_ptr(), ld, out.data_ptr(), M, E, vocab, scale,
               -1 if pad_idx is None else pad_idx, int(accumulate), ws.data_ptr(), need)
     return out
+
+
+def _vector(t, name, E):
+    if t is not None:
+        _dense(t, name, (E,), torch.float32)
+
+
+def _gate(gate, M, E, dtype):
+    """(type code, rows) of a gate [E] or [G, E] with G dividing M; (f32, 0) for none."""
+    if gate is None:
+        return TC_F32, 0
+    _dense(gate, "gate")
+    G = 1 if gate.dim() == 1 else gate.shape[0]
+    if gate.dim() not in (1, 2) or gate.shape[-1] != E or G == 0 or M % G:
+        raise ValueError(f"gate of shape {tuple(gate.shape)} for {M} rows of {E}: [E] or [G, E] with G dividing the rows")
+    if gate.dtype != torch.float32 and gate.dtype != dtype:
+        raise TypeError(f"gate has type {gate.dtype}, expected float32 or {dtype}")
+    return _dt(gate), G
+
+
+def gated_residual_norm(y, x, post_gamma, post_beta=None, gate=None, pre_gamma=None, pre_beta=None, res_scale=1.0, eps=1e-5,
+                        rms=False):
+    """The end of a block and the start of the next in one pass over y (the block's output, [M, E] f32 or bf16) and the f32
+    residual stream x [M, E]:
+
+        x_out = res_scale * x + gate * norm(y; post)        h = norm(x_out; pre)
+
+    norm: LayerNorm, or root-mean-square norm with ``rms``; betas are optional.  gate: None, [E], or [G, E] whose row g is for rows
+    g M/G .. (g+1) M/G - 1 (one per sequence, or one per row).  Without ``pre_gamma`` there is no h.
+    Returns (x_out f32, h of y's type or None, stats f32 [M, 4] for the backward pass).  tc_gated_residual_norm_fwd."""
+    dev = _same_device(y, x, post_gamma, post_beta, gate, pre_gamma, pre_beta)
+    dt, ldy, ldx = _dt(y), _rows(y, "y"), _rows(x, "x")
+    M, E = y.shape
+    if x.shape != y.shape or x.dtype != torch.float32:
+        raise ValueError(f"x must be float32 {tuple(y.shape)}, got {x.dtype} {tuple(x.shape)}")
+    for t, n in ((post_gamma, "post_gamma"), (post_beta, "post_beta"), (pre_gamma, "pre_gamma"), (pre_beta, "pre_beta")):
+        _vector(t, n, E)
+    if pre_gamma is None and pre_beta is not None:
+        raise ValueError("pre_beta without pre_gamma")
+    gdt, G = _gate(gate, M, E, y.dtype)
+    x_out = torch.empty(M, E, dtype=torch.float32, device=dev)
+    h = None if pre_gamma is None else torch.empty(M, E, dtype=y.dtype, device=dev)
+    stats = torch.empty(M, 4, dtype=torch.float32, device=dev)
+    if M and E:
+        _call("tc_gated_residual_norm_fwd", dev, dt, y.data_ptr(), ldy, x.data_ptr(), ldx, post_gamma.data_ptr(), _p(post_beta),
+              gdt, _p(gate), G, res_scale, _p(pre_gamma), _p(pre_beta), x_out.data_ptr(), _p(h), stats.data_ptr(), M, E, int(rms),
+              eps, eps)
+    return x_out, h, stats
+
+
+def gated_residual_norm_bwd(dh, dx_out, y, x_out, stats, post_gamma, post_beta=None, gate=None, pre_gamma=None, pre_beta=None,
+                            res_scale=1.0, rms=False, into=None):
+    """Gradient of :func:`gated_residual_norm`: dh (of y's type) and dx_out (f32) are those of h and x_out, either may be None
+    (dh is None exactly where there is no second norm); y, x_out and stats are those of the forward pass.
+
+    Returns (dy, dx, d_post_gamma, d_post_beta, d_gate, d_pre_gamma, d_pre_beta), f32 but for dy, None where there is no such
+    vector.  into: five f32 buffers or None in the order of the last five, which are added to instead.
+    tc_gated_residual_norm_bwd."""
+    dev = _same_device(dh, dx_out, y, x_out, stats, post_gamma, post_beta, gate, pre_gamma, pre_beta, *(into or ()))
+    dt, ldy, ldx = _dt(y), _rows(y, "y"), _rows(x_out, "x_out")
+    M, E = y.shape
+    if x_out.shape != y.shape or x_out.dtype != torch.float32:
+        raise ValueError(f"x_out must be float32 {tuple(y.shape)}, got {x_out.dtype} {tuple(x_out.shape)}")
+    if (dh is None) != (pre_gamma is None):
+        raise ValueError("dh and pre_gamma go together")
+    if dh is None and dx_out is None:
+        raise ValueError("neither dh nor dx_out")
+    if dh is not None and (dh.shape != y.shape or dh.dtype != y.dtype):
+        raise ValueError(f"dh must be {y.dtype} {tuple(y.shape)}, got {dh.dtype} {tuple(dh.shape)}")
+    if dx_out is not None and (dx_out.shape != y.shape or dx_out.dtype != torch.float32):
+        raise ValueError(f"dx_out must be float32 {tuple(y.shape)}, got {dx_out.dtype} {tuple(dx_out.shape)}")
+    _dense(stats, "stats", (M, 4), torch.float32)
+    for t, n in ((post_gamma, "post_gamma"), (post_beta, "post_beta"), (pre_gamma, "pre_gamma"), (pre_beta, "pre_beta")):
+        _vector(t, n, E)
+    gdt, G = _gate(gate, M, E, y.dtype)
+    dy = torch.empty(M, E, dtype=y.dtype, device=dev)
+    dx = torch.empty(M, E, dtype=torch.float32, device=dev)
+    vectors = (post_gamma, post_beta, gate, pre_gamma, pre_beta)
+    got, accumulate = [], 0
+    for v, given, bit in zip(vectors, into or (None,) * 5, (1, 2, 16, 4, 8)):
+        if given is not None:
+            if v is None:
+                raise ValueError("into has a buffer for a vector that is not there")
+            _dense(given, "buffer in into", v.shape, torch.float32)
+            accumulate |= bit
+        elif v is not None:
+            given = (torch.empty if M and E else torch.zeros)(v.shape, dtype=torch.float32, device=dev)
+        got.append(given)
+    if M and E:
+        need = _lib.load().tc_gated_residual_norm_bwd_workspace_bytes(M, E, G)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        d_post_gamma, d_post_beta, d_gate, d_pre_gamma, d_pre_beta = got
+        _call("tc_gated_residual_norm_bwd", dev, dt, _p(dh), 0 if dh is None else _rows(dh, "dh"), _p(dx_out),
+              0 if dx_out is None else _rows(dx_out, "dx_out"), y.data_ptr(), ldy, x_out.data_ptr(), ldx, stats.data_ptr(),
+              post_gamma.data_ptr(), _p(post_beta), gdt, _p(gate), G, res_scale, _p(pre_gamma), dy.data_ptr(), dx.data_ptr(),
+              _p(d_post_gamma), _p(d_post_beta), _p(d_gate), _p(d_pre_gamma), _p(d_pre_beta), accumulate, M, E, int(rms),
+              ws.data_ptr(), need)
+    return (dy, dx, *got)
