@@ -739,6 +739,29 @@ int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh, const floa
                                float *d_gate, float *d_pre_gamma, float *d_pre_beta, int accumulate, long M, int E, int rms,
                                void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- activations kept for the backward pass in 8 bits ------------------------------------------------
+ * Each run of 32 values along a row (the last run of a row may be shorter) shares a power of two 2^e, kept as the byte
+ * e + 127 (e8m0); a value v is kept as the OCP e4m3 number nearest to v / 2^e (ties to even).  2^e is the smallest power of
+ * two, at least 2^-126, with which no finite value of the run passes 448.  Infinities and NaN become NaN and do not
+ * count for e.  codes [M,E] and scales [M, ceil(E/32)], a byte each, dense: E + E/32 bytes a row instead of 2 E (bf16).
+ * x, u, dy: dtype f32 or bf16, row strides >= E; act, du, out: dtype, dense.  E <= 2^20.
+ */
+int tc_act8_pack(int dtype, const void *x, long ldx, void *codes, void *scales, long M, int E, void *stream);
+int tc_act8_unpack(int dtype, const void *codes, const void *scales, void *out, long M, int E, void *stream);
+/* act = gelu(u) (exact erf form, transcodon/modules.py:17-24) and the 8-bit form of u in one pass */
+int tc_gelu_act8(int dtype, const void *u, long ldu, void *act, void *codes, void *scales, long M, int E, void *stream);
+/* du = dy * gelu'(v) and, unless act is NULL, act = gelu(v), v being what the codes stand for.  du may be dy (dense). */
+int tc_dgelu_act8(int dtype, const void *dy, long ld_dy, const void *codes, const void *scales, void *du, void *act, long M, int E,
+                  void *stream);
+/*
+ * Weight gradient of a linear layer whose input is kept in 8 bits: dW[N,K] (+)= sum over m of dy[m,n] * v[m,k], f32, on the
+ * matrix cores; v enters exactly.  dy [M,N] bf16 with row stride ld_dy, codes [M,K], scales [M, ceil(K/32)] dense; N and
+ * ld_dy multiples of 8, K of 16; 16-byte aligned.  The sum has a fixed order.
+ */
+size_t tc_gemm_tn_act8_workspace_bytes(long M, int N, int K);            /* 0: unsupported shape */
+int tc_gemm_tn_act8(const void *dy, long ld_dy, const void *codes, const void *scales, float *dW, long M, int N, int K,
+                    int accumulate, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -158,6 +158,12 @@ _SIGNATURES = {
     "tc_gated_residual_norm_bwd": (C.c_int, [C.c_int, vp, C.c_long, vp, C.c_long, vp, C.c_long, vp, C.c_long, vp, vp, vp,
                                              C.c_int, vp, C.c_int, C.c_float, vp, vp, vp, vp, vp, vp, vp, vp, C.c_int,
                                              C.c_long, C.c_int, C.c_int, vp, C.c_size_t, vp]),
+    "tc_act8_pack": (C.c_int, [C.c_int, vp, C.c_long, vp, vp, C.c_long, C.c_int, vp]),
+    "tc_act8_unpack": (C.c_int, [C.c_int, vp, vp, vp, C.c_long, C.c_int, vp]),
+    "tc_gelu_act8": (C.c_int, [C.c_int, vp, C.c_long, vp, vp, vp, C.c_long, C.c_int, vp]),
+    "tc_dgelu_act8": (C.c_int, [C.c_int, vp, C.c_long, vp, vp, vp, vp, C.c_long, C.c_int, vp]),
+    "tc_gemm_tn_act8_workspace_bytes": (C.c_size_t, [C.c_long, C.c_int, C.c_int]),
+    "tc_gemm_tn_act8": (C.c_int, [vp, C.c_long, vp, vp, vp, C.c_long, C.c_int, C.c_int, C.c_int, vp, C.c_size_t, vp]),
     "tc_prof_enable": (C.c_int, [C.c_int]),
     "tc_prof_reset": (C.c_int, []),
     "tc_prof_collect": (C.c_int, [C.c_int, C.POINTER(C.c_int64), C.POINTER(C.c_double),

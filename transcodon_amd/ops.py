@@ -520,3 +520,99 @@ def gated_residual_norm_bwd(dh, dx_out, y, x_out, stats, post_gamma, post_beta=N
               _p(d_post_gamma), _p(d_post_beta), _p(d_gate), _p(d_pre_gamma), _p(d_pre_beta), accumulate, M, E, int(rms),
               ws.data_ptr(), need)
     return (dy, dx, *got)
+
+
+ACT8_GROUP = 32      # neighbouring values of a row that share a scale
+
+
+def _act8(codes, scales):
+    """(M, E) of an 8-bit activation: codes float8_e4m3fn [M, E], scales float8_e8m0fnu [M, ceil(E / 32)]."""
+    if codes.dim() != 2:
+        raise ValueError("codes must be [M, E]")
+    M, E = codes.shape
+    _dense(codes, "codes", dtype=torch.float8_e4m3fn)
+    _dense(scales, "scales", (M, (E + ACT8_GROUP - 1) // ACT8_GROUP), torch.float8_e8m0fnu)
+    return M, E
+
+
+def _act8_empty(M, E, dev):
+    return (torch.empty(M, E, dtype=torch.float8_e4m3fn, device=dev),
+            torch.empty(M, (E + ACT8_GROUP - 1) // ACT8_GROUP, dtype=torch.float8_e8m0fnu, device=dev))
+
+
+def act8_pack(x):
+    """8-bit form of an activation x [M, E] (f32 or bf16, rows may be strided) kept for the backward pass: codes
+    (float8_e4m3fn [M, E]) and scales (float8_e8m0fnu, one power of two per row and 32 columns); a value is
+    code * scale, at most half an e4m3 step from x.  tc_act8_pack."""
+    dev = _same_device(x)
+    dt, ld = _dt(x), _rows(x, "x")
+    M, E = x.shape
+    codes, scales = _act8_empty(M, E, dev)
+    if M and E:
+        _call("tc_act8_pack", dev, dt, x.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), M, E)
+    return codes, scales
+
+
+def act8_unpack(codes, scales, out_dtype=torch.bfloat16):
+    """The values of an 8-bit activation, [M, E] f32 or bf16 (exact in both but below 2^-133 in bf16).  tc_act8_unpack."""
+    dev = _same_device(codes, scales)
+    M, E = _act8(codes, scales)
+    out = torch.empty(M, E, dtype=out_dtype, device=dev)
+    dt = _dt(out)
+    if M and E:
+        _call("tc_act8_unpack", dev, dt, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), M, E)
+    return out
+
+
+def gelu_act8(u):
+    """(gelu(u) in u's type, codes, scales): the activation of a feed-forward block and the 8-bit form of its input in one pass
+    over u [M, E].  tc_gelu_act8."""
+    dev = _same_device(u)
+    dt, ld = _dt(u), _rows(u, "u")
+    M, E = u.shape
+    act = torch.empty(M, E, dtype=u.dtype, device=dev)
+    codes, scales = _act8_empty(M, E, dev)
+    if M and E:
+        _call("tc_gelu_act8", dev, dt, u.data_ptr(), ld, act.data_ptr(), codes.data_ptr(), scales.data_ptr(), M, E)
+    return act, codes, scales
+
+
+def dgelu_act8(dy, codes, scales, want_act=False):
+    """dy * gelu'(v) in dy's type, v being the values of the 8-bit activation; with ``want_act`` also gelu(v), which the weight
+    gradient of the next linear layer reads, from the same pass.  tc_dgelu_act8."""
+    dev = _same_device(dy, codes, scales)
+    dt, ld = _dt(dy), _rows(dy, "dy")
+    M, E = _act8(codes, scales)
+    if dy.shape != (M, E):
+        raise ValueError(f"dy has shape {tuple(dy.shape)}, the codes {(M, E)}")
+    du = torch.empty(M, E, dtype=dy.dtype, device=dev)
+    act = torch.empty(M, E, dtype=dy.dtype, device=dev) if want_act else None
+    if M and E:
+        _call("tc_dgelu_act8", dev, dt, dy.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), du.data_ptr(), _p(act), M, E)
+    return (du, act) if want_act else du
+
+
+def gemm_tn_act8(dy, codes, scales, out=None):
+    """Weight gradient dy^T v -> f32 [N, K] of a linear layer whose input v [M, K] is kept in 8 bits (added to ``out`` when given);
+    dy [M, N] bf16, rows may be strided; N a multiple of 8, K of 16.  tc_gemm_tn_act8."""
+    dev = _same_device(dy, codes, scales, out)
+    if dy.dtype != torch.bfloat16:
+        raise TypeError(f"dy must be bfloat16, got {dy.dtype}")
+    ld = _rows(dy, "dy")
+    M, K = _act8(codes, scales)
+    N = dy.shape[1]
+    if dy.shape[0] != M:
+        raise ValueError(f"dy has {dy.shape[0]} rows, the codes {M}")
+    accumulate = out is not None
+    if accumulate:
+        _dense(out, "out", (N, K), torch.float32)
+    elif M == 0:
+        return torch.zeros(N, K, dtype=torch.float32, device=dev)
+    else:
+        out = torch.empty(N, K, dtype=torch.float32, device=dev)
+    if M:
+        need = _lib.load().tc_gemm_tn_act8_workspace_bytes(M, N, K)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        _call("tc_gemm_tn_act8", dev, dy.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), M, N, K,
+              int(accumulate), ws.data_ptr(), need)
+    return out
