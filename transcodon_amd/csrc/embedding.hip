@@ -42,127 +42,230 @@ __global__ __launch_bounds__(256) void embedding_kernel(const TID *__restrict__ 
     }
 }
 
+// ---- gradient of a few positions -----------------------------------------------------------------------
+// Up to kFew positions: no sort.  Every wave holds all ids, finds the positions of a table row by comparing, and adds their
+// rows of dy in order; rows without a position are written as zeros on the way.
+constexpr int kFew = 256;
+struct FewParams {
+    const void *tokens, *dy;
+    float *out;
+    long ld_dy, vocab, pad_idx;
+    int M, E, accumulate;
+    float scale;
+};
+template <typename T, typename TID, int VEC>
+__global__ __launch_bounds__(256) void few_positions_kernel(const FewParams p) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = blockIdx.y * 64 * VEC + lane * VEC;
+    const bool in = col < p.E;
+    long id[kFew / 64];
+#pragma unroll
+    for (int k = 0; k < kFew / 64; ++k) {
+        const int i = k * 64 + lane;
+        id[k] = i < p.M ? (long)static_cast<const TID *>(p.tokens)[i] : -1;
+        if (id[k] == p.pad_idx) id[k] = -1;
+    }
+    for (long v = (long)blockIdx.x * 4 + wave; v < p.vocab; v += (long)gridDim.x * 4) {
+        float acc[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+        bool any = false;
+#pragma unroll
+        for (int k = 0; k < kFew / 64; ++k) {
+            unsigned long long left = __ballot(id[k] == v);
+            any |= left != 0;
+            while (left) {
+                constexpr int U = 8;                               // rows in flight; a spent mask repeats its last row
+                int at[U], n = 0;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (left) {
+                        at[u] = __ffsll((long long)left) - 1;
+                        left &= left - 1;
+                        n = u + 1;
+                    } else {
+                        at[u] = at[u > 0 ? u - 1 : 0];
+                    }
+                }
+                float x[U][VEC];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (in) tc_load_row<T, VEC>(static_cast<const T *>(p.dy) + (long)(k * 64 + at[u]) * p.ld_dy + col, x[u]);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (u < n)
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) acc[j] += x[u][j];
+            }
+        }
+        if (!in || (p.accumulate && !any)) continue;
+        float *dst = p.out + v * p.E + col, old[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) old[j] = 0.f;
+        if (p.accumulate) tc_load_row<float, VEC>(dst, old);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] = old[j] + p.scale * acc[j];
+        tc_store_row<float, VEC>(dst, acc);
+    }
+}
+
 // ---- stable radix sort of the token positions ------------------------------------------------------------
-// Key of a position: its id, or `vocab` (sorts last, ignored by the sums) for padding and ids out of range.
-constexpr int kSortTile = 1024;       // positions a workgroup sorts per pass while there are few
+// Key of a position: its id, or `vocab` (sorts last, ignored by the sums) for padding and ids out of range.  Digits of at
+// most 9 bits from the lowest up; per digit one launch counts every workgroup's positions and a second places them behind
+// all smaller digits and all earlier equal ones.  (Counting the next digit with atomics while the present one is placed
+// saves a launch, but frequent ids meet on one counter: 65 us instead of 10 at 49153 positions.)  Up to 4096 positions are
+// one workgroup's work and all digits one launch.  The sort keeps few CUs busy, so its launches also clear the gradient,
+// a slice each, with workgroups of their own.
+constexpr int kSortWaves = 16;
+constexpr int kSortTile = 4096;       // positions of a workgroup while there are few: 4 rounds of each wave
 constexpr int kMaxBlocks = 256;
 constexpr int kMaxBits = 9;
 
 struct SortParams {
     const void *tokens;               // first pass: ids (4 or 8 bytes each)
-    const uint32_t *keys_in, *pos_in; // later passes
-    uint32_t *keys_out, *pos_out;
+    uint32_t *keys[2], *pos[2];       // later passes: from [(pass - 1) & 1] to [pass & 1]
     uint32_t *hist;                   // [blocks][bins]
-    int id_bytes;                     // 0: keys_in / pos_in
-    int M, tile, shift, bits;
+    int id_bytes, M, tile, blocks, bits, passes;
     long vocab, pad_idx;
+    float *clear;                     // gradient to clear (null: none), this launch's slice
+    long clear_from, clear_to;
 };
 
-__device__ __forceinline__ uint32_t sort_key(const SortParams &p, int i) {
-    if (p.id_bytes == 0) return p.keys_in[i];
+__device__ __forceinline__ uint32_t sort_key(const SortParams &p, int pass, int i) {
+    if (pass > 0) return p.keys[(pass - 1) & 1][i];
     const long tok = p.id_bytes == 8 ? static_cast<const long *>(p.tokens)[i] : (long)static_cast<const int32_t *>(p.tokens)[i];
     return tok == p.pad_idx || tok < 0 || tok >= p.vocab ? (uint32_t)p.vocab : (uint32_t)tok;
 }
 
-__global__ __launch_bounds__(256) void sort_hist_kernel(const SortParams p) {
-    __shared__ uint32_t h[1 << kMaxBits];
-    const int bins = 1 << p.bits;
-    for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
-    __syncthreads();
-    const int begin = blockIdx.x * p.tile, end = min(p.M, begin + p.tile);
-    for (int i = begin + threadIdx.x; i < end; i += 256) atomicAdd(&h[(sort_key(p, i) >> p.shift) & (bins - 1)], 1u);
-    __syncthreads();
-    for (int d = threadIdx.x; d < bins; d += 256) p.hist[(long)blockIdx.x * bins + d] = h[d];
+// true for the workgroups behind the sorting ones, after they have cleared their part
+__device__ __forceinline__ bool clear_slice(const SortParams &p) {
+    if ((int)blockIdx.x < p.blocks) return false;
+    const long n = p.clear_to - p.clear_from, step = (long)(gridDim.x - p.blocks) * 64 * kSortWaves;
+    float *out = p.clear + p.clear_from;
+    const long first = (long)(blockIdx.x - p.blocks) * 64 * kSortWaves + threadIdx.x;
+    if (((uintptr_t)out & 15) == 0) {
+        for (long i = first; i < n / 4; i += step) *reinterpret_cast<f32x4 *>(out + 4 * i) = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (long i = n / 4 * 4 + first; i < n; i += step) out[i] = 0.f;
+    } else {
+        for (long i = first; i < n; i += step) out[i] = 0.f;
+    }
+    return true;
 }
 
-// Where this workgroup's positions of digit d go: all positions of smaller digits, then those of the same digit in
-// earlier workgroups, earlier waves of this one, earlier lanes.
-__global__ __launch_bounds__(256) void sort_scatter_kernel(const SortParams p) {
-    __shared__ uint32_t at[4][1 << kMaxBits];      // next place per wave and digit
+__global__ __launch_bounds__(64 * kSortWaves) void sort_count_kernel(const SortParams p, int pass) {
+    if (clear_slice(p)) return;
+    __shared__ uint32_t h[1 << kMaxBits];
+    const int bins = 1 << p.bits;
+    for (int d = threadIdx.x; d < bins; d += 64 * kSortWaves) h[d] = 0;
+    __syncthreads();
+    const int begin = blockIdx.x * p.tile, end = min(p.M, begin + p.tile);
+    for (int i = begin + threadIdx.x; i < end; i += 64 * kSortWaves) atomicAdd(&h[(sort_key(p, pass, i) >> (pass * p.bits)) & (bins - 1)], 1u);
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += 64 * kSortWaves) p.hist[(long)blockIdx.x * bins + d] = h[d];
+}
+
+__global__ __launch_bounds__(64 * kSortWaves) void sort_place_kernel(const SortParams p, int first_pass, int last_pass) {
+    if (clear_slice(p)) return;
+    __shared__ uint32_t at[kSortWaves][1 << kMaxBits];      // next place per wave and digit
     __shared__ uint32_t total[1 << kMaxBits];
     const int bins = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int begin = blockIdx.x * p.tile, end = min(p.M, begin + p.tile);
-    const int span = p.tile / 4;                   // tile is a multiple of 256
+    const int span = p.tile / kSortWaves;                    // the tile is a multiple of 64 kSortWaves
     const int w_begin = begin + wave * span, w_end = min(end, w_begin + span);
-    for (int d = threadIdx.x; d < 4 * bins; d += 256) at[d >> p.bits][d & (bins - 1)] = 0;
-    __syncthreads();
-    for (int i = w_begin + lane; i < w_end; i += 64) atomicAdd(&at[wave][(sort_key(p, i) >> p.shift) & (bins - 1)], 1u);
-    uint32_t before[2] = {0, 0};                   // bins <= 512: at most two digits per thread
-    for (int k = 0, d = threadIdx.x; d < bins; d += 256, ++k) {
-        uint32_t sum = 0, mine = 0;
-#pragma unroll 8
-        for (int b = 0; b < (int)gridDim.x; ++b) {
-            if (b == (int)blockIdx.x) mine = sum;
-            sum += p.hist[(long)b * bins + d];
+    for (int pass = first_pass; pass <= last_pass; ++pass) { // more than one only where there is one workgroup
+        const int shift = pass * p.bits;
+        for (int d = threadIdx.x; d < kSortWaves * bins; d += 64 * kSortWaves) at[d >> p.bits][d & (bins - 1)] = 0;
+        __syncthreads();
+        for (int i = w_begin + lane; i < w_end; i += 64) atomicAdd(&at[wave][(sort_key(p, pass, i) >> shift) & (bins - 1)], 1u);
+        uint32_t before = 0;                                 // bins <= 512: at most one digit per thread
+        const int d = threadIdx.x;
+        if (p.blocks > 1 && d < bins) {
+            uint32_t sum = 0;
+            const uint32_t *h = p.hist + d;
+#pragma unroll 16
+            for (int b = 0; b < p.blocks; ++b) {
+                const uint32_t n = h[(long)b * bins];
+                before += b < (int)blockIdx.x ? n : 0;
+                sum += n;
+            }
+            total[d] = sum;
         }
-        total[d] = sum;
-        before[k] = mine;
-    }
-    __syncthreads();
-    // exclusive scan of the totals by one wave, eight digits per lane
-    if (wave == 0) {
-        uint32_t v[8], s = 0;
+        __syncthreads();
+        if (p.blocks == 1 && d < bins) {
+            uint32_t sum = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int d = lane * 8 + j;
-            v[j] = s;
-            s += d < bins ? total[d] : 0;
+            for (int w = 0; w < kSortWaves; ++w) sum += at[w][d];
+            total[d] = sum;
         }
-        uint32_t incl = s;
+        __syncthreads();
+        // exclusive scan of the totals by one wave, eight digits per lane
+        if (wave == 0) {
+            uint32_t v[8], s = 0;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t o = __shfl_up(incl, off, 64);
-            if (lane >= off) incl += o;
-        }
+            for (int j = 0; j < 8; ++j) {
+                v[j] = s;
+                s += lane * 8 + j < bins ? total[lane * 8 + j] : 0;
+            }
+            uint32_t incl = s;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int d = lane * 8 + j;
-            if (d < bins) total[d] = incl - s + v[j];
-        }
-    }
-    __syncthreads();
-    for (int k = 0, d = threadIdx.x; d < bins; d += 256, ++k) {
-        uint32_t place = total[d] + before[k];
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t o = __shfl_up(incl, off, 64);
+                if (lane >= off) incl += o;
+            }
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t n = at[w][d];
-            at[w][d] = place;
-            place += n;
+            for (int j = 0; j < 8; ++j)
+                if (lane * 8 + j < bins) total[lane * 8 + j] = incl - s + v[j];
         }
-    }
-    __syncthreads();
-    for (int i0 = w_begin; i0 < w_end; i0 += 64) {
-        const int i = i0 + lane;
-        const bool live = i < w_end;
-        const uint32_t key = live ? sort_key(p, i) : 0;
-        const uint32_t digit = (key >> p.shift) & (bins - 1);
-        unsigned long long same = __ballot(live);
-        for (int b = 0; b < p.bits; ++b) {
-            const unsigned long long ones = __ballot((digit >> b) & 1u);
-            same &= ((digit >> b) & 1u) ? ones : ~ones;
+        __syncthreads();
+        if (d < bins) {
+            uint32_t place = total[d] + before;
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) {
+                const uint32_t n = at[w][d];
+                at[w][d] = place;
+                place += n;
+            }
         }
-        // the first lane of each digit moves the wave's place on by the number of its lanes
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        uint32_t place = 0;
-        if (live && rank == 0) place = atomicAdd(&at[wave][digit], (uint32_t)__popcll(same));
-        const int first = same ? __ffsll((long long)same) - 1 : 0;
-        place = __shfl(place, first, 64) + rank;
-        if (live) {
-            p.keys_out[place] = key;
-            p.pos_out[place] = p.id_bytes ? (uint32_t)i : p.pos_in[i];
+        __syncthreads();
+        uint32_t *keys_out = p.keys[pass & 1], *pos_out = p.pos[pass & 1];
+        for (int i0 = w_begin; i0 < w_end; i0 += 64) {
+            const int i = i0 + lane;
+            const bool live = i < w_end;
+            const uint32_t key = live ? sort_key(p, pass, i) : 0;
+            const uint32_t digit = (key >> shift) & (bins - 1);
+            unsigned long long same = __ballot(live);
+            for (int b = 0; b < p.bits; ++b) {
+                const unsigned long long ones = __ballot((digit >> b) & 1u);
+                same &= ((digit >> b) & 1u) ? ones : ~ones;
+            }
+            // the first lane of each digit moves the wave's place on by the number of its lanes
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            uint32_t place = 0;
+            if (live && rank == 0) place = atomicAdd(&at[wave][digit], (uint32_t)__popcll(same));
+            const int first = same ? __ffsll((long long)same) - 1 : 0;
+            place = __shfl(place, first, 64) + rank;
+            if (live) {
+                keys_out[place] = key;
+                pos_out[place] = pass == 0 ? (uint32_t)i : p.pos[(pass - 1) & 1][i];
+            }
         }
+        __syncthreads();                                     // the next pass of the same workgroup reads what all its waves wrote
     }
 }
 
 // ---- segmented sum ----------------------------------------------------------------------------------------
+// A workgroup takes kSumWaves pieces of kPiece positions; each wave sums the runs of its piece, and where a run goes on into
+// the next piece the sums are handed over in LDS.  What crosses the workgroup's ends goes to memory, one row at either
+// end, for segment_join_kernel.
+constexpr int kSumWaves = 8, kPiece = 32, kSpan = kSumWaves * kPiece;
 struct SumParams {
     const uint32_t *keys, *pos;       // sorted
     const void *dy;
     long ld_dy;
     float *out;                       // [vocab, E]
-    float *partial;                   // [pieces][2][part_ld]: run from the piece before, run into the piece after
+    float *partial;                   // [spans][2][part_ld]: run from the span before, run into the span after
     int part_ld;
-    int M, E, piece, pieces, accumulate;
+    int M, E, spans, accumulate;
     uint32_t vocab;
     float scale;
 };
@@ -182,98 +285,136 @@ __device__ __forceinline__ void write_row(const SumParams &p, uint32_t key, int 
     tc_store_row<float, VEC>(dst, v);
 }
 
-// One wave: one piece of the sorted list (at most 64 positions) x 64 VEC columns.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void segment_sum_kernel(const SumParams p) {
-    const int lane = threadIdx.x & 63;
-    const int c = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slab = blockIdx.y;
-    if (c >= p.pieces) return;
-    const int begin = c * p.piece, n = min(p.piece, p.M - begin);
-    const int mine = begin + min(lane, n - 1);
-    const int keys = (int)p.keys[mine], pos = (int)p.pos[mine];
-    const int before = begin > 0 ? (int)p.keys[begin - 1] : -1;
-    const int after = begin + n < p.M ? (int)p.keys[begin + n] : -1;
-    const int col = slab * 64 * VEC + lane * VEC;
+__global__ __launch_bounds__(64 * kSumWaves) void segment_sum_kernel(const SumParams p) {
+    __shared__ float rows[kSumWaves][2][VEC][64];            // [wave][run from before / run into after]
+    __shared__ int open[kSumWaves];                          // bit 0: a run comes from before, 1: one goes on, 2: they are the same
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int begin = blockIdx.x * kSpan + wave * kPiece, n = min(kPiece, p.M - begin);      // n <= 0: nothing left
+    const int col = blockIdx.y * 64 * VEC + lane * VEC;
     const bool in = col < p.E;
-    float acc[VEC];
+    int flags = 0, first_key = -1, last_key = -1;
+    if (n > 0) {
+        const int mine = begin + min(lane, n - 1);
+        const int keys = (int)p.keys[mine], pos = (int)p.pos[mine];
+        const int before = begin > 0 ? (int)p.keys[begin - 1] : -1;
+        const int after = begin + n < p.M ? (int)p.keys[begin + n] : -1;
+        first_key = __builtin_amdgcn_readfirstlane(keys);
+        last_key = __builtin_amdgcn_readlane(keys, n - 1);
+        // padding and ids out of range fill the end of the list
+        const int live = __popcll(__ballot(lane < n && (uint32_t)keys != p.vocab));
+        if (live > 0 && before == first_key) flags |= 1;
+        if (live == n && after == last_key) flags |= 2;
+        float acc[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-    int run = 0;                                   // where the current run starts in the piece
-    constexpr int U = 8;                           // rows in flight
-    for (int i0 = 0; i0 < n; i0 += U) {
-        float v[U][VEC];
+        for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+        int run = 0;                                         // where the current run starts in the piece
+        constexpr int U = 8;                                 // rows in flight
+        for (int i0 = 0; i0 < live; i0 += U) {
+            float v[U][VEC];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = __builtin_amdgcn_readlane(pos, min(i0 + u, n - 1));
-            if (in) tc_load_row<T, VEC>(static_cast<const T *>(p.dy) + (long)(uint32_t)at * p.ld_dy + col, v[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + u;
-            if (i >= n) break;
-            const int key = __builtin_amdgcn_readlane(keys, i);
-            if ((uint32_t)key == p.vocab) return;  // padding and ids out of range fill the end of the list
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] += v[u][j];
-            const int next = i + 1 < n ? __builtin_amdgcn_readlane(keys, i + 1) : after;
-            if (next == key && i + 1 < n) continue;
-            const bool from_before = run == 0 && before == key, into_after = next == key;
-            if (in) {
-                if (!from_before && !into_after) write_row<VEC>(p, (uint32_t)key, col, acc);
-                else tc_store_row<float, VEC>(p.partial + ((long)c * 2 + (from_before ? 0 : 1)) * p.part_ld + col, acc);
+            for (int u = 0; u < U; ++u) {
+                const int at = __builtin_amdgcn_readlane(pos, min(i0 + u, live - 1));
+                if (in) tc_load_row<T, VEC>(static_cast<const T *>(p.dy) + (long)(uint32_t)at * p.ld_dy + col, v[u]);
             }
-            run = i + 1;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + u;
+                if (i >= live) break;
+                const int key = __builtin_amdgcn_readlane(keys, i);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] += v[u][j];
+                if (i + 1 < n && __builtin_amdgcn_readlane(keys, min(i + 1, 63)) == key) continue;
+                const bool from_before = run == 0 && (flags & 1), into_after = i + 1 == n && (flags & 2);
+                if (from_before || into_after) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) rows[wave][from_before ? 0 : 1][j][lane] = acc[j];
+                    if (from_before && into_after) flags |= 4;
+                } else if (in) {
+                    write_row<VEC>(p, (uint32_t)key, col, acc);
+                }
+                run = i + 1;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+            }
         }
+    }
+    if (lane == 0) open[wave] = flags;
+    __syncthreads();
+    // Runs that leave a piece: the wave in which such a run starts (for a run from before the workgroup: wave 0) adds the
+    // parts of the waves that follow, in order.
+    const bool from_before = wave == 0 && (flags & 1), starts = (flags & 2) && !(flags & 4);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        if (which == 0 ? !from_before : !starts) continue;
+        float acc[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] = rows[wave][which][j][lane];
+        bool goes_on = which == 1 || (flags & 4);
+        for (int w = wave + 1; w < kSumWaves && goes_on; ++w) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) acc[j] += rows[w][0][j][lane];
+            goes_on = (open[w] & 4) != 0;
+        }
+        if (!in) continue;
+        if (which == 1 && !goes_on) write_row<VEC>(p, (uint32_t)last_key, col, acc);
+        else tc_store_row<float, VEC>(p.partial + ((long)blockIdx.x * 2 + which) * p.part_ld + col, acc);
     }
 }
 
-// Runs over several pieces: the wave of the piece in which the run starts adds the partial rows in order.
+// Runs over several spans: the wave of the span in which the run starts adds the rows in order.
 template <int VEC>
 __global__ __launch_bounds__(256) void segment_join_kernel(const SumParams p) {
     const int lane = threadIdx.x & 63;
-    const int c = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slab = blockIdx.y;
-    if (c + 1 >= p.pieces) return;
-    const int begin = c * p.piece;
-    const uint32_t key = p.keys[begin + p.piece - 1];
-    if (key == p.vocab || p.keys[begin + p.piece] != key) return;
-    if (begin > 0 && p.keys[begin - 1] == key) return;           // starts earlier
-    const int col = slab * 64 * VEC + lane * VEC;
-    const bool in = col < p.E;
-    float acc[VEC], v[VEC];
+    const int c = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (c + 1 >= p.spans) return;
+    const long begin = (long)c * kSpan;
+    const uint32_t key = p.keys[begin + kSpan - 1];
+    if (key == p.vocab || p.keys[begin + kSpan] != key) return;
+    if (begin > 0 && p.keys[begin - 1] == key) return;       // starts earlier
+    const int col = blockIdx.y * 64 * VEC + lane * VEC;
+    float acc[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    const bool in = col < p.E;
     if (in) tc_load_row<float, VEC>(p.partial + ((long)c * 2 + 1) * p.part_ld + col, acc);
-    for (int k = c + 1; k < p.pieces && p.keys[k * p.piece] == key; ++k) {
-        if (!in) continue;
-        tc_load_row<float, VEC>(p.partial + (long)k * 2 * p.part_ld + col, v);
+    for (int k0 = c + 1; k0 < p.spans; k0 += 64) {
+        // the spans that begin inside the run follow each other without a gap
+        const int k = k0 + lane;
+        const int n = __popcll(__ballot(k < p.spans && p.keys[(long)min(k, p.spans - 1) * kSpan] == key));
+        constexpr int U = 8;
+        for (int i = 0; i < n && in; i += U) {
+            float v[U][VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += v[j];
+            for (int u = 0; u < U; ++u) tc_load_row<float, VEC>(p.partial + (long)(k0 + min(i + u, n - 1)) * 2 * p.part_ld + col, v[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u < n)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) acc[j] += v[u][j];
+        }
+        if (n < 64) break;
     }
     if (in) write_row<VEC>(p, key, col, acc);
 }
 
-__global__ __launch_bounds__(256) void fill_zero_kernel(float *__restrict__ out, long n) {
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) out[i] = 0.f;
-}
-
 struct BwdPlan {
-    int tile, blocks, passes, bits, piece, pieces, part_ld;
+    int tile, blocks, passes, bits, spans, part_ld;
     size_t keys[2], pos[2], hist, partial, total;
 };
 BwdPlan bwd_plan(long M, long E, long vocab) {
     BwdPlan w{};
+    if (M <= kFew) { w.total = 16; return w; }
+    const long unit = 64 * kSortWaves;
     long tile = (M + kMaxBlocks - 1) / kMaxBlocks;
-    tile = (tile + 255) / 256 * 256;
+    tile = (tile + unit - 1) / unit * unit;
     w.tile = (int)(tile < kSortTile ? kSortTile : tile);
     w.blocks = (int)((M + w.tile - 1) / w.tile);
     int bits = 0;
     while ((vocab >> bits) != 0) ++bits;           // keys 0 .. vocab
     w.passes = (bits + kMaxBits - 1) / kMaxBits;
     w.bits = (bits + w.passes - 1) / w.passes;
-    w.piece = 64;
-    w.pieces = (int)((M + w.piece - 1) / w.piece);
+    w.spans = (int)((M + kSpan - 1) / kSpan);
     w.part_ld = (int)((E + 3) / 4 * 4);
     size_t off = 0;
     auto take = [&](size_t bytes) {
@@ -283,7 +424,7 @@ BwdPlan bwd_plan(long M, long E, long vocab) {
     };
     for (int k = 0; k < 2; ++k) { w.keys[k] = take((size_t)M * 4); w.pos[k] = take((size_t)M * 4); }
     w.hist = take((size_t)w.blocks * (1 << w.bits) * 4);
-    w.partial = take((size_t)w.pieces * 2 * w.part_ld * 4);
+    w.partial = take((size_t)w.spans * 2 * w.part_ld * 4);
     w.total = off;
     return w;
 }
@@ -360,48 +501,81 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
     if (pad_idx < 0) pad_idx = INT64_MIN;
     char *ws = static_cast<char *>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool vec = tc_rows_aligned(dy, ld_dy, esz, 4) && tc_rows_aligned(d_table, E, 4, 4);
+    const unsigned slabs = (unsigned)((E + (vec ? 255 : 63)) / (vec ? 256 : 64));
+#define TC_EMB_T(KERNEL, GRID, BLOCK, P)                                                                                        \
+    do {                                                                                                                        \
+        if (dy_dtype == TC_F32) {                                                                                               \
+            if (vec) TC_LAUNCH((KERNEL(float, 4)), GRID, dim3(BLOCK), 0, s, P);                                                 \
+            else TC_LAUNCH((KERNEL(float, 1)), GRID, dim3(BLOCK), 0, s, P);                                                     \
+        } else {                                                                                                                \
+            if (vec) TC_LAUNCH((KERNEL(uint16_t, 4)), GRID, dim3(BLOCK), 0, s, P);                                              \
+            else TC_LAUNCH((KERNEL(uint16_t, 1)), GRID, dim3(BLOCK), 0, s, P);                                                  \
+        }                                                                                                                       \
+    } while (0)
+    if (M <= kFew) {
+        FewParams f{};
+        f.tokens = tokens; f.dy = dy; f.out = d_table; f.ld_dy = ld_dy; f.vocab = vocab; f.pad_idx = pad_idx;
+        f.M = (int)M; f.E = E; f.accumulate = accumulate; f.scale = scale;
+        const long want = (vocab + 3) / 4, most = 8192 / slabs > 256 ? 8192 / slabs : 256;
+        const dim3 grid((unsigned)(want < most ? want : most), slabs);
+#define TC_FEW4(T, V) few_positions_kernel<T, int32_t, V>
+#define TC_FEW8(T, V) few_positions_kernel<T, int64_t, V>
+        if (id_bytes == 4) TC_EMB_T(TC_FEW4, grid, 256, f);
+        else TC_EMB_T(TC_FEW8, grid, 256, f);
+        TC_CHECK_LAUNCH("tc_embedding_bwd");
+        return TC_OK;
+    }
     SortParams sp{};
     sp.tokens = tokens;
     sp.id_bytes = id_bytes;
-    sp.M = (int)M; sp.tile = w.tile; sp.bits = w.bits;
+    sp.M = (int)M; sp.tile = w.tile; sp.blocks = w.blocks; sp.bits = w.bits; sp.passes = w.passes;
     sp.vocab = vocab; sp.pad_idx = pad_idx;
     sp.hist = reinterpret_cast<uint32_t *>(ws + w.hist);
+    for (int k = 0; k < 2; ++k) {
+        sp.keys[k] = reinterpret_cast<uint32_t *>(ws + w.keys[k]);
+        sp.pos[k] = reinterpret_cast<uint32_t *>(ws + w.pos[k]);
+    }
+    // the launches of the sort clear a slice of the gradient each, 64 KiB and more per workgroup
+    const int launches = w.blocks == 1 ? 1 : 2 * w.passes;
+    const long cells = accumulate ? 0 : vocab * E;
+    int launch = 0;
+    auto grid_of = [&]() {
+        sp.clear = d_table;
+        sp.clear_from = cells / 4 * launch / launches * 4;
+        ++launch;
+        sp.clear_to = launch == launches ? cells : cells / 4 * launch / launches * 4;
+        const long wgs = (sp.clear_to - sp.clear_from + 16383) / 16384;
+        return dim3((unsigned)(w.blocks + (wgs < 512 ? wgs : 512)));
+    };
     for (int pass = 0; pass < w.passes; ++pass) {
-        sp.shift = pass * w.bits;
-        sp.keys_out = reinterpret_cast<uint32_t *>(ws + w.keys[pass & 1]);
-        sp.pos_out = reinterpret_cast<uint32_t *>(ws + w.pos[pass & 1]);
-        TC_LAUNCH(sort_hist_kernel, dim3(w.blocks), dim3(256), 0, s, sp);
-        TC_LAUNCH(sort_scatter_kernel, dim3(w.blocks), dim3(256), 0, s, sp);
-        sp.id_bytes = 0;
-        sp.keys_in = sp.keys_out;
-        sp.pos_in = sp.pos_out;
+        dim3 grid = grid_of();
+        if (w.blocks == 1) {
+            TC_LAUNCH(sort_place_kernel, grid, dim3(64 * kSortWaves), 0, s, sp, 0, w.passes - 1);
+            break;
+        }
+        TC_LAUNCH(sort_count_kernel, grid, dim3(64 * kSortWaves), 0, s, sp, pass);
+        grid = grid_of();
+        TC_LAUNCH(sort_place_kernel, grid, dim3(64 * kSortWaves), 0, s, sp, pass, pass);
     }
     SumParams q{};
-    q.keys = sp.keys_in; q.pos = sp.pos_in;
+    q.keys = sp.keys[(w.passes - 1) & 1]; q.pos = sp.pos[(w.passes - 1) & 1];
     q.dy = dy; q.ld_dy = ld_dy;
     q.out = d_table;
     q.partial = reinterpret_cast<float *>(ws + w.partial);
     q.part_ld = w.part_ld;
-    q.M = (int)M; q.E = E; q.piece = w.piece; q.pieces = w.pieces;
+    q.M = (int)M; q.E = E; q.spans = w.spans;
     q.accumulate = accumulate; q.vocab = (uint32_t)vocab; q.scale = scale;
-    const bool vec = tc_rows_aligned(dy, ld_dy, esz, 4) && tc_rows_aligned(d_table, E, 4, 4);
-    const dim3 blocks((w.pieces + 3) / 4, (E + (vec ? 255 : 63)) / (vec ? 256 : 64));
-    if (!accumulate) {
-        const long n = vocab * E;
-        const long most = 4096;
-        TC_LAUNCH(fill_zero_kernel, dim3((unsigned)((n + 255) / 256 < most ? (n + 255) / 256 : most)), dim3(256), 0, s, d_table, n);
+#define TC_SUM(T, V) segment_sum_kernel<T, V>
+    TC_EMB_T(TC_SUM, dim3((unsigned)w.spans, slabs), 64 * kSumWaves, q);
+    if (w.spans > 1) {
+        if (vec) TC_LAUNCH(segment_join_kernel<4>, dim3((unsigned)(w.spans + 3) / 4, slabs), dim3(256), 0, s, q);
+        else TC_LAUNCH(segment_join_kernel<1>, dim3((unsigned)(w.spans + 3) / 4, slabs), dim3(256), 0, s, q);
     }
-    if (dy_dtype == TC_F32) {
-        if (vec) TC_LAUNCH((segment_sum_kernel<float, 4>), blocks, dim3(256), 0, s, q);
-        else TC_LAUNCH((segment_sum_kernel<float, 1>), blocks, dim3(256), 0, s, q);
-    } else {
-        if (vec) TC_LAUNCH((segment_sum_kernel<uint16_t, 4>), blocks, dim3(256), 0, s, q);
-        else TC_LAUNCH((segment_sum_kernel<uint16_t, 1>), blocks, dim3(256), 0, s, q);
-    }
-    if (w.pieces > 1) {
-        if (vec) TC_LAUNCH(segment_join_kernel<4>, blocks, dim3(256), 0, s, q);
-        else TC_LAUNCH(segment_join_kernel<1>, blocks, dim3(256), 0, s, q);
-    }
+#undef TC_SUM
+#undef TC_FEW8
+#undef TC_FEW4
+#undef TC_EMB_T
     TC_CHECK_LAUNCH("tc_embedding_bwd");
     return TC_OK;
 }

@@ -340,15 +340,20 @@ def _same_device(*tensors):
     return dev
 
 
+# handle of a device's current stream without a Stream object around it (2 us of a call's 7)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def _call(name, dev, *args):
     """One library call on ``dev``'s current stream, also where another device is the current one."""
     fn = getattr(_lib.load(), name)
     if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        rc = fn(*args, _raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    check(rc, name)
+            rc = fn(*args, _raw_stream(dev.index))
+    if rc:
+        check(rc, name)
 
 
 def _rows(t, name):
