@@ -198,7 +198,7 @@ def test_gradient_is_that_of_differences():
 
 @gpu
 @pytest.mark.parametrize("M,N,K", [(1, 8, 16), (1, 128, 128), (63, 8, 48), (64, 136, 112), (65, 128, 256), (131, 264, 80), (262, 768, 768),
-                                   (1000, 96, 1040), (4097, 256, 256), (8192, 512, 768), (8200, 776, 784)])
+                                   (1000, 96, 1040), (4097, 256, 256), (8192, 512, 768), (8200, 776, 784), (8192, 2304, 768), (8197, 2304, 776 + 8), (3400, 4096, 4096)])
 def test_weight_gradient(M, N, K):
     gen = torch.Generator().manual_seed(M + N + K)
     dy = torch.randn(M, N, generator=gen).bfloat16()
@@ -219,6 +219,23 @@ def test_weight_gradient(M, N, K):
     wide = torch.full((M, N + 16), float("nan"), dtype=torch.bfloat16, device=DEV)          # a NaN beside the rows is not read into them
     wide[:, 8:8 + N] = dy.to(DEV)
     assert torch.equal(ops.gemm_tn_act8(wide[:, 8:8 + N], codes, scales), got)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 128 * 64])
+def test_weight_gradient_of_one_row_is_the_row(rows):
+    """One row of ones among rows of zeros: every value of the activation comes out as it is, whatever its code and scale."""
+    N, K = 2048, 1024
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    bits = bits[torch.isfinite(bits.float())]
+    for first in range(0, 65280 - K + 1, 9 * K):
+        x = torch.ones(rows, K, dtype=torch.bfloat16)
+        x[rows // 2] = bits[first:first + K]
+        dy = torch.zeros(rows, N, dtype=torch.bfloat16, device=DEV)
+        dy[rows // 2] = 1.0
+        codes, scales = ops.act8_pack(x.to(DEV))
+        want = ops.act8_unpack(codes[rows // 2:rows // 2 + 1], scales[rows // 2:rows // 2 + 1], torch.float32)
+        assert torch.equal(ops.gemm_tn_act8(dy, codes, scales), want.expand(N, K))
 
 
 @gpu
@@ -265,8 +282,8 @@ def test_refusals_without_a_gpu():
     assert lib.tc_gelu_act8(0, one, 8, None, one, one, 4, 8, None) == -1
     assert lib.tc_act8_unpack(0, one, one, None, 4, 8, None) == lib.tc_act8_unpack(0, one, one, one + 1, 4, 8, None) == -1
     assert lib.tc_dgelu_act8(0, one, 7, one, one, one, None, 4, 8, None) == lib.tc_dgelu_act8(0, one, 8, one, one, None, None, 4, 8, None) == -1
-    need = lib.tc_gemm_tn_act8_workspace_bytes(4, 8, 16)
-    assert need > 0 and lib.tc_gemm_tn_act8_workspace_bytes(4, 4, 16) == lib.tc_gemm_tn_act8_workspace_bytes(4, 8, 8) == 0
+    need = lib.tc_gemm_tn_act8_workspace_bytes(4, 8, 8, 16)
+    assert need > 0 and lib.tc_gemm_tn_act8_workspace_bytes(4, 4, 4, 16) == lib.tc_gemm_tn_act8_workspace_bytes(4, 8, 8, 8) == 0
     tn = lambda dy=one, ld=8, codes=one, dW=one, M=4, N=8, K=16, ws=one, n=need: lib.tc_gemm_tn_act8(dy, ld, codes, one, dW, M, N, K, 0, ws, n, None)
     for bad in (dict(dy=None), dict(ld=4), dict(ld=12), dict(dy=one + 2), dict(codes=one + 8), dict(N=12), dict(K=24), dict(M=0), dict(ws=None)):
         assert tn(**bad) == -1, bad

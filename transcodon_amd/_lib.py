@@ -162,7 +162,7 @@ _SIGNATURES = {
     "tc_act8_unpack": (C.c_int, [C.c_int, vp, vp, vp, C.c_long, C.c_int, vp]),
     "tc_gelu_act8": (C.c_int, [C.c_int, vp, C.c_long, vp, vp, vp, C.c_long, C.c_int, vp]),
     "tc_dgelu_act8": (C.c_int, [C.c_int, vp, C.c_long, vp, vp, vp, vp, C.c_long, C.c_int, vp]),
-    "tc_gemm_tn_act8_workspace_bytes": (C.c_size_t, [C.c_long, C.c_int, C.c_int]),
+    "tc_gemm_tn_act8_workspace_bytes": (C.c_size_t, [C.c_long, C.c_long, C.c_int, C.c_int]),
     "tc_gemm_tn_act8": (C.c_int, [vp, C.c_long, vp, vp, vp, C.c_long, C.c_int, C.c_int, C.c_int, vp, C.c_size_t, vp]),
     "tc_prof_enable": (C.c_int, [C.c_int]),
     "tc_prof_reset": (C.c_int, []),

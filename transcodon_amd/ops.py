@@ -616,7 +616,7 @@ def gemm_tn_act8(dy, codes, scales, out=None):
     else:
         out = torch.empty(N, K, dtype=torch.float32, device=dev)
     if M:
-        need = _lib.load().tc_gemm_tn_act8_workspace_bytes(M, N, K)
+        need = _lib.load().tc_gemm_tn_act8_workspace_bytes(M, ld, N, K)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
         _call("tc_gemm_tn_act8", dev, dy.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), M, N, K,
               int(accumulate), ws.data_ptr(), need)
