@@ -4,8 +4,9 @@
 //   tc_gelu_act8     u -> gelu(u), codes and scales of u                        (forward)
 //   tc_dgelu_act8    dy, codes, scales -> dy * gelu'(u8), gelu(u8) again        (backward; u8: what the codes stand for)
 //
-// A lane owns 8 neighbouring values of a row, four lanes a run of 32; rows that do not fit (width or alignment) go one
-// value a lane, 32 lanes a run.  Everything is one pass over memory.
+// A lane owns 8 neighbouring values of a row, four lanes a run of 32.  Where rows follow each other without a gap and hold
+// whole runs, a piece's place is its number (FLAT); otherwise lanes are dealt to rows, addresses may be aligned to single
+// elements only, and a row's last values go one by one.  Everything is one pass over memory.
 #include "act8.h"
 #include "row_io.h"
 
@@ -30,149 +31,147 @@ __device__ __forceinline__ float normal_cdf(float x, float &e) {
     return x < 0.f ? q : 1.0f - q;
 }
 
+constexpr int VEC = 8;
+constexpr int kLanesPerRun = kAct8Group / VEC;
+
 struct Act8Params {
     const void *x;           // u, x or dy
     long ldx;
     void *y;                 // act, du or the unpacked values; dense
     void *again;             // gelu of the checkpoint (may be null)
     uint8_t *codes, *scales;
-    long n_pieces;           // rows * pieces per row
-    int E, groups, pieces;   // width, runs per row, pieces (of VEC values) per row
+    long rows, n_pieces;     // n_pieces (FLAT): rows * E / VEC
+    int E, groups;           // width, runs per row
+    int lanes_log2;          // not FLAT: lanes of a row, at least those of a run
 };
 
 // largest magnitude bits over the lanes of a run
-template <int VEC>
 __device__ __forceinline__ uint32_t run_max(uint32_t m) {
-    if constexpr (VEC == 8) {
-        m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));     // lane ^ 1
-        m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));     // lane ^ 2
-    } else {
-#pragma unroll
-        for (int off = 1; off < kAct8Group; off <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, 64));
-    }
-    return m;
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));     // lane ^ 1
+    return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));  // lane ^ 2
 }
 
-template <int VEC>
-__device__ __forceinline__ void store_codes(uint8_t *dst, const float (&v)[VEC]) {
-    if constexpr (VEC == 8) {
-        u32x2 w;
+template <bool LOOSE>
+__device__ __forceinline__ void store_codes(uint8_t *dst, const float (&v)[VEC], int n) {
+    u32x2 w;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k], v[4 * k + 1], 0, false);
-            c = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2], v[4 * k + 3], c, true);
-            w[k] = (uint32_t)c;
-        }
+    for (int k = 0; k < 2; ++k) {
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k], v[4 * k + 1], 0, false);
+        c = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2], v[4 * k + 3], c, true);
+        w[k] = (uint32_t)c;
+    }
+    if constexpr (!LOOSE) {
         *reinterpret_cast<u32x2 *>(dst) = w;
+    } else if (n >= VEC) {
+        __builtin_memcpy(dst, &w, VEC);
     } else {
-        *dst = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[0], 0, false);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (j < n) dst[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
     }
 }
 
-template <int VEC>
-__device__ __forceinline__ void load_codes(const uint8_t *src, float (&v)[VEC]) {
-    if constexpr (VEC == 8) {
-        const u32x2 w = *reinterpret_cast<const u32x2 *>(src);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], true);
-            v[4 * k] = lo[0]; v[4 * k + 1] = lo[1]; v[4 * k + 2] = hi[0]; v[4 * k + 3] = hi[1];
-        }
+template <bool LOOSE>
+__device__ __forceinline__ void load_codes(const uint8_t *src, float (&v)[VEC], int n) {
+    u32x2 w = u32x2{0u, 0u};
+    if constexpr (!LOOSE) {
+        w = *reinterpret_cast<const u32x2 *>(src);
+    } else if (n >= VEC) {
+        __builtin_memcpy(&w, src, VEC);
     } else {
-        v[0] = __builtin_amdgcn_cvt_pk_f32_fp8((int)*src, false)[0];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (j < n) w[j >> 2] |= (uint32_t)src[j] << (8 * (j & 3));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], true);
+        v[4 * k] = lo[0]; v[4 * k + 1] = lo[1]; v[4 * k + 2] = hi[0]; v[4 * k + 3] = hi[1];
     }
 }
 
-// T: type of x and y.  FLAT: rows follow each other without a gap and hold whole runs, so a piece's place is its number.
-template <typename T, int VEC, bool FLAT, bool GELU>
-__global__ __launch_bounds__(256) void act8_pack_kernel(const Act8Params p) {
-    constexpr int LPG = kAct8Group / VEC;                         // lanes per run
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < p.n_pieces; i += (long)gridDim.x * 256) {
-        long row = 0, at_x, at;
-        int col = 0;
-        bool in = true;
-        if constexpr (FLAT) {
-            at_x = at = i * VEC;
-        } else {
-            row = i / p.pieces;
-            col = (int)(i - row * p.pieces) * VEC;
-            in = col < p.E;
-            at_x = row * p.ldx + col;
-            at = row * p.E + col;
-        }
-        float v[VEC];
+// One piece: x and the dense outputs at at_x and at, n of its values are there (0 .. VEC; all four lanes of a run call this).
+template <typename T, bool LOOSE, bool GELU>
+__device__ __forceinline__ void pack_piece(const Act8Params &p, long at_x, long at, long run, int n) {
+    float v[VEC], w[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = 0.f;
-        if (in) tc_load_row<T, VEC>(static_cast<const T *>(p.x) + at_x, v);
-        uint32_t m = 0;
+    for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+    if (!LOOSE || n > 0) tc_load_row<T, VEC, LOOSE>(static_cast<const T *>(p.x) + at_x, v, n);
+    uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) m = max(m, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
-        m = run_max<VEC>(m);
-        float w[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] = v[j];
-        if (m >= 0x7f800000u) {                                    // some value is not finite (the whole run comes here)
-            m = 0;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const uint32_t b = __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu;
-                if (b < 0x7f800000u) m = max(m, b);
-                else w[j] = __builtin_nanf("");
-            }
-            m = run_max<VEC>(m);
-        }
-        const int byte = act8_scale_byte(m);
-        const float inv = act8_inverse(byte);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] *= inv;
-        if (in) {
-            store_codes<VEC>(p.codes + at, w);
-            if constexpr (GELU) {
-                float e;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] *= normal_cdf(v[j], e);
-                tc_store_row<T, VEC>(static_cast<T *>(p.y) + at, v);
-            }
-        }
-        if ((threadIdx.x & (LPG - 1)) == 0) p.scales[FLAT ? i / LPG : row * p.groups + col / kAct8Group] = (uint8_t)byte;
+    for (int j = 0; j < VEC; ++j) {
+        m = max(m, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
+        w[j] = v[j];
     }
+    m = run_max(m);
+    if (m >= 0x7f800000u) {                                    // some value is not finite (the whole run comes here)
+        m = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const uint32_t b = __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu;
+            if (b < 0x7f800000u) m = max(m, b);
+            else w[j] = __builtin_nanf("");
+        }
+        m = run_max(m);
+    }
+    const int byte = act8_scale_byte(m);
+    const float inv = act8_inverse(byte);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) w[j] *= inv;
+    if (!LOOSE || n > 0) {
+        store_codes<LOOSE>(p.codes + at, w, n);
+        if constexpr (GELU) {
+            float e;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] *= normal_cdf(v[j], e);
+            tc_store_row<T, VEC, LOOSE>(static_cast<T *>(p.y) + at, v, n);
+        }
+    }
+    if ((threadIdx.x & (kLanesPerRun - 1)) == 0) p.scales[run] = (uint8_t)byte;
 }
 
 // GELU: x is dy, y is du; otherwise y receives the values that the codes stand for
-template <typename T, int VEC, bool FLAT, bool GELU>
-__global__ __launch_bounds__(256) void act8_read_kernel(const Act8Params p) {
-    constexpr int LPG = kAct8Group / VEC;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < p.n_pieces; i += (long)gridDim.x * 256) {
-        long row = 0, at_x, at;
-        int col = 0;
-        if constexpr (FLAT) {
-            at_x = at = i * VEC;
-        } else {
-            row = i / p.pieces;
-            col = (int)(i - row * p.pieces) * VEC;
-            if (col >= p.E) continue;
-            at_x = row * p.ldx + col;
-            at = row * p.E + col;
+template <typename T, bool LOOSE, bool GELU>
+__device__ __forceinline__ void read_piece(const Act8Params &p, long at_x, long at, long run, int n) {
+    if (LOOSE && n <= 0) return;
+    float v[VEC], d[VEC];
+    load_codes<LOOSE>(p.codes + at, v, n);
+    const float scale = act8_scale(p.scales[run]);
+    if constexpr (GELU) tc_load_row<T, VEC, LOOSE>(static_cast<const T *>(p.x) + at_x, d, n);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] *= scale;
+    if constexpr (GELU) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            float e;
+            const float cdf = normal_cdf(v[j], e);
+            d[j] *= fmaf(v[j] * 0.3989422804014327f, e, cdf);  // Phi(u) + u phi(u)
+            v[j] *= cdf;
         }
-        float v[VEC], d[VEC];
-        load_codes<VEC>(p.codes + at, v);
-        const float scale = act8_scale(p.scales[FLAT ? i / LPG : row * p.groups + col / kAct8Group]);
-        if constexpr (GELU) tc_load_row<T, VEC>(static_cast<const T *>(p.x) + at_x, d);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] *= scale;
-        if constexpr (GELU) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                float e;
-                const float cdf = normal_cdf(v[j], e);
-                d[j] *= fmaf(v[j] * 0.3989422804014327f, e, cdf);  // Phi(u) + u phi(u)
-                v[j] *= cdf;
+        tc_store_row<T, VEC, LOOSE>(static_cast<T *>(p.y) + at, d, n);
+        if (p.again) tc_store_row<T, VEC, LOOSE>(static_cast<T *>(p.again) + at, v, n);
+    } else {
+        tc_store_row<T, VEC, LOOSE>(static_cast<T *>(p.y) + at, v, n);
+    }
+}
+
+template <typename T, bool FLAT, bool GELU, bool READ>
+__global__ __launch_bounds__(256) void act8_kernel(const Act8Params p) {
+    if constexpr (FLAT) {
+        for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < p.n_pieces; i += (long)gridDim.x * 256) {
+            if constexpr (READ) read_piece<T, false, GELU>(p, i * VEC, i * VEC, i / kLanesPerRun, VEC);
+            else pack_piece<T, false, GELU>(p, i * VEC, i * VEC, i / kLanesPerRun, VEC);
+        }
+    } else {
+        const int sub = threadIdx.x & ((1 << p.lanes_log2) - 1);
+        const long step = ((long)gridDim.x * 256) >> p.lanes_log2;
+        for (long row = ((long)blockIdx.x * 256 + threadIdx.x) >> p.lanes_log2; row < p.rows; row += step)
+            // the lanes of a run stay together: the run's first column decides
+            for (int col = sub * VEC; (col & ~(kAct8Group - 1)) < p.E; col += VEC << p.lanes_log2) {
+                const long run = row * p.groups + col / kAct8Group;
+                if constexpr (READ) read_piece<T, true, GELU>(p, row * p.ldx + col, row * p.E + col, run, p.E - col);
+                else pack_piece<T, true, GELU>(p, row * p.ldx + col, row * p.E + col, run, p.E - col);
             }
-            tc_store_row<T, VEC>(static_cast<T *>(p.y) + at, d);
-            if (p.again) tc_store_row<T, VEC>(static_cast<T *>(p.again) + at, v);
-        } else {
-            tc_store_row<T, VEC>(static_cast<T *>(p.y) + at, v);
-        }
     }
 }
 
@@ -182,32 +181,32 @@ int act8_check(const char *who, int dtype, long M, int E) {
     return TC_OK;
 }
 
-Act8Params act8_params(const void *x, long ldx, void *y, void *again, void *codes, void *scales, long M, int E, int esz, bool &vec,
-                       bool &flat) {
+Act8Params act8_params(const void *x, long ldx, void *y, void *again, void *codes, void *scales, long M, int E, int esz, bool &flat) {
     Act8Params p{};
     p.x = x; p.ldx = ldx; p.y = y; p.again = again;
     p.codes = static_cast<uint8_t *>(codes);
     p.scales = static_cast<uint8_t *>(scales);
     p.E = E;
     p.groups = (E + kAct8Group - 1) / kAct8Group;
-    vec = E % 8 == 0 && (!x || tc_rows_aligned(x, ldx, esz, 8)) && (!y || tc_rows_aligned(y, E, esz, 8)) &&
-          (!again || tc_rows_aligned(again, E, esz, 8)) && (uintptr_t)codes % 8 == 0;
-    flat = E % kAct8Group == 0 && (!x || ldx == E);
-    p.pieces = p.groups * (kAct8Group / (vec ? 8 : 1));
-    p.n_pieces = M * p.pieces;
+    p.rows = M;
+    p.n_pieces = M * (E / VEC);
+    p.lanes_log2 = 2;
+    while (p.lanes_log2 < 8 && (VEC << p.lanes_log2) < E) ++p.lanes_log2;
+    flat = E % kAct8Group == 0 && (!x || (ldx == E && tc_rows_aligned(x, E, esz, VEC))) && tc_rows_aligned(y, E, esz, VEC) &&
+           tc_rows_aligned(again, E, esz, VEC) && (uintptr_t)codes % VEC == 0;
     return p;
 }
 
-dim3 act8_grid(const Act8Params &p) {
-    const long blocks = (p.n_pieces + 255) / 256, most = 1L << 20;      // a launch holds fewer than 2^32 threads
+dim3 act8_grid(const Act8Params &p, bool flat) {
+    const long lanes = flat ? p.n_pieces : p.rows << p.lanes_log2;
+    const long blocks = (lanes + 255) / 256, most = 1L << 20;      // a launch holds fewer than 2^32 threads
     return dim3((unsigned)(blocks < most ? blocks : most));
 }
 
-#define TC_A8(KERNEL, T, GELU)                                                                                          \
+#define TC_A8(T, GELU, READ)                                                                                            \
     do {                                                                                                                \
-        if (vec && flat) TC_LAUNCH((KERNEL<T, 8, true, GELU>), act8_grid(p), dim3(256), 0, s, p);                       \
-        else if (vec) TC_LAUNCH((KERNEL<T, 8, false, GELU>), act8_grid(p), dim3(256), 0, s, p);                         \
-        else TC_LAUNCH((KERNEL<T, 1, false, GELU>), act8_grid(p), dim3(256), 0, s, p);                                  \
+        if (flat) TC_LAUNCH((act8_kernel<T, true, GELU, READ>), act8_grid(p, true), dim3(256), 0, s, p);                \
+        else TC_LAUNCH((act8_kernel<T, false, GELU, READ>), act8_grid(p, false), dim3(256), 0, s, p);                   \
     } while (0)
 
 int pack_call(const char *who, int dtype, const void *x, long ldx, void *act, void *codes, void *scales, long M, int E, bool gelu,
@@ -218,12 +217,12 @@ int pack_call(const char *who, int dtype, const void *x, long ldx, void *act, vo
     TC_REQUIRE(x && codes && scales && (act || !gelu), "%s: null operand", who);
     TC_REQUIRE(ldx >= E && ((uintptr_t)x | (uintptr_t)act) % esz == 0, "%s: bad row stride or alignment", who);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    bool vec, flat;
-    const Act8Params p = act8_params(x, ldx, act, nullptr, codes, scales, M, E, esz, vec, flat);
+    bool flat;
+    const Act8Params p = act8_params(x, ldx, act, nullptr, codes, scales, M, E, esz, flat);
     if (dtype == TC_F32) {
-        if (gelu) TC_A8(act8_pack_kernel, float, true); else TC_A8(act8_pack_kernel, float, false);
+        if (gelu) TC_A8(float, true, false); else TC_A8(float, false, false);
     } else {
-        if (gelu) TC_A8(act8_pack_kernel, uint16_t, true); else TC_A8(act8_pack_kernel, uint16_t, false);
+        if (gelu) TC_A8(uint16_t, true, false); else TC_A8(uint16_t, false, false);
     }
     TC_CHECK_LAUNCH(who);
     return TC_OK;
@@ -245,10 +244,10 @@ extern "C" int tc_act8_unpack(int dtype, const void *codes, const void *scales, 
     const int esz = dtype == TC_BF16 ? 2 : 4;
     TC_REQUIRE(codes && scales && out && (uintptr_t)out % esz == 0, "tc_act8_unpack: null or misaligned operand");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    bool vec, flat;
-    const Act8Params p = act8_params(nullptr, 0, out, nullptr, const_cast<void *>(codes), const_cast<void *>(scales), M, E, esz, vec, flat);
-    if (dtype == TC_F32) TC_A8(act8_read_kernel, float, false);
-    else TC_A8(act8_read_kernel, uint16_t, false);
+    bool flat;
+    const Act8Params p = act8_params(nullptr, 0, out, nullptr, const_cast<void *>(codes), const_cast<void *>(scales), M, E, esz, flat);
+    if (dtype == TC_F32) TC_A8(float, false, true);
+    else TC_A8(uint16_t, false, true);
     TC_CHECK_LAUNCH("tc_act8_unpack");
     return TC_OK;
 }
@@ -261,10 +260,10 @@ extern "C" int tc_dgelu_act8(int dtype, const void *dy, long ld_dy, const void *
     TC_REQUIRE(dy && codes && scales && du, "tc_dgelu_act8: null operand");
     TC_REQUIRE(ld_dy >= E && ((uintptr_t)dy | (uintptr_t)du | (uintptr_t)act) % esz == 0, "tc_dgelu_act8: bad row stride or alignment");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    bool vec, flat;
-    const Act8Params p = act8_params(dy, ld_dy, du, act, const_cast<void *>(codes), const_cast<void *>(scales), M, E, esz, vec, flat);
-    if (dtype == TC_F32) TC_A8(act8_read_kernel, float, true);
-    else TC_A8(act8_read_kernel, uint16_t, true);
+    bool flat;
+    const Act8Params p = act8_params(dy, ld_dy, du, act, const_cast<void *>(codes), const_cast<void *>(scales), M, E, esz, flat);
+    if (dtype == TC_F32) TC_A8(float, true, true);
+    else TC_A8(uint16_t, true, true);
     TC_CHECK_LAUNCH("tc_dgelu_act8");
     return TC_OK;
 }

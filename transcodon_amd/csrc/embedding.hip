@@ -14,7 +14,7 @@ namespace {
 
 // ---- lookup ------------------------------------------------------------------------------------------
 // 2^lanes_log2 lanes (at most a wave) share a row.
-template <typename TT, typename TO, typename TID, int VEC>
+template <typename TT, typename TO, typename TID, int VEC, bool LOOSE>
 __global__ __launch_bounds__(256) void embedding_kernel(const TID *__restrict__ tokens, const TT *__restrict__ table,
                                                         TO *__restrict__ out, long M, int E, long vocab, float scale,
                                                         long pad_idx, int lanes_log2, int32_t *bad) {
@@ -33,14 +33,16 @@ __global__ __launch_bounds__(256) void embedding_kernel(const TID *__restrict__ 
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) v[j] = 0.f;
             } else {
-                tc_load_row<TT, VEC>(src + c, v);
+                tc_load_row<TT, VEC, LOOSE>(src + c, v, E - c);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) v[j] *= scale;      // in f32, rounded once by the store
             }
-            tc_store_row<TO, VEC>(dst + c, v);
+            tc_store_row<TO, VEC, LOOSE>(dst + c, v, E - c);
         }
     }
 }
+
+constexpr int VEC = 4;                // columns of a lane in the gradient's kernels; a wave takes 64 VEC columns
 
 // ---- gradient of a few positions -----------------------------------------------------------------------
 // Up to kFew positions: no sort.  Every wave holds all ids, finds the positions of a table row by comparing, and adds their
@@ -53,7 +55,7 @@ struct FewParams {
     int M, E, accumulate;
     float scale;
 };
-template <typename T, typename TID, int VEC>
+template <typename T, typename TID, bool LOOSE>
 __global__ __launch_bounds__(256) void few_positions_kernel(const FewParams p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = blockIdx.y * 64 * VEC + lane * VEC;
@@ -90,7 +92,7 @@ __global__ __launch_bounds__(256) void few_positions_kernel(const FewParams p) {
                 float x[U][VEC];
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (in) tc_load_row<T, VEC>(static_cast<const T *>(p.dy) + (long)(k * 64 + at[u]) * p.ld_dy + col, x[u]);
+                    if (in) tc_load_row<T, VEC, LOOSE>(static_cast<const T *>(p.dy) + (long)(k * 64 + at[u]) * p.ld_dy + col, x[u], p.E - col);
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (u < n)
@@ -102,10 +104,10 @@ __global__ __launch_bounds__(256) void few_positions_kernel(const FewParams p) {
         float *dst = p.out + v * p.E + col, old[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) old[j] = 0.f;
-        if (p.accumulate) tc_load_row<float, VEC>(dst, old);
+        if (p.accumulate) tc_load_row<float, VEC, LOOSE>(dst, old, p.E - col);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) acc[j] = old[j] + p.scale * acc[j];
-        tc_store_row<float, VEC>(dst, acc);
+        tc_store_row<float, VEC, LOOSE>(dst, acc, p.E - col);
     }
 }
 
@@ -270,22 +272,22 @@ struct SumParams {
     float scale;
 };
 
-template <int VEC>
+template <bool LOOSE>
 __device__ __forceinline__ void write_row(const SumParams &p, uint32_t key, int col, const float (&acc)[VEC]) {
     float v[VEC];
     float *dst = p.out + (long)key * p.E + col;
     if (p.accumulate) {
-        tc_load_row<float, VEC>(dst, v);
+        tc_load_row<float, VEC, LOOSE>(dst, v, p.E - col);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[j] += p.scale * acc[j];
     } else {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[j] = p.scale * acc[j];
     }
-    tc_store_row<float, VEC>(dst, v);
+    tc_store_row<float, VEC, LOOSE>(dst, v, p.E - col);
 }
 
-template <typename T, int VEC>
+template <typename T, bool LOOSE>
 __global__ __launch_bounds__(64 * kSumWaves) void segment_sum_kernel(const SumParams p) {
     __shared__ float rows[kSumWaves][2][VEC][64];            // [wave][run from before / run into after]
     __shared__ int open[kSumWaves];                          // bit 0: a run comes from before, 1: one goes on, 2: they are the same
@@ -315,7 +317,7 @@ __global__ __launch_bounds__(64 * kSumWaves) void segment_sum_kernel(const SumPa
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int at = __builtin_amdgcn_readlane(pos, min(i0 + u, live - 1));
-                if (in) tc_load_row<T, VEC>(static_cast<const T *>(p.dy) + (long)(uint32_t)at * p.ld_dy + col, v[u]);
+                if (in) tc_load_row<T, VEC, LOOSE>(static_cast<const T *>(p.dy) + (long)(uint32_t)at * p.ld_dy + col, v[u], p.E - col);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(64 * kSumWaves) void segment_sum_kernel(const SumPa
                     for (int j = 0; j < VEC; ++j) rows[wave][from_before ? 0 : 1][j][lane] = acc[j];
                     if (from_before && into_after) flags |= 4;
                 } else if (in) {
-                    write_row<VEC>(p, (uint32_t)key, col, acc);
+                    write_row<LOOSE>(p, (uint32_t)key, col, acc);
                 }
                 run = i + 1;
 #pragma unroll
@@ -357,13 +359,13 @@ __global__ __launch_bounds__(64 * kSumWaves) void segment_sum_kernel(const SumPa
             goes_on = (open[w] & 4) != 0;
         }
         if (!in) continue;
-        if (which == 1 && !goes_on) write_row<VEC>(p, (uint32_t)last_key, col, acc);
+        if (which == 1 && !goes_on) write_row<LOOSE>(p, (uint32_t)last_key, col, acc);
         else tc_store_row<float, VEC>(p.partial + ((long)blockIdx.x * 2 + which) * p.part_ld + col, acc);
     }
 }
 
 // Runs over several spans: the wave of the span in which the run starts adds the rows in order.
-template <int VEC>
+template <bool LOOSE>
 __global__ __launch_bounds__(256) void segment_join_kernel(const SumParams p) {
     const int lane = threadIdx.x & 63;
     const int c = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -395,7 +397,7 @@ __global__ __launch_bounds__(256) void segment_join_kernel(const SumParams p) {
         }
         if (n < 64) break;
     }
-    if (in) write_row<VEC>(p, key, col, acc);
+    if (in) write_row<LOOSE>(p, key, col, acc);
 }
 
 struct BwdPlan {
@@ -447,30 +449,30 @@ extern "C" int tc_embedding_fwd(int table_dtype, int out_dtype, int id_bytes, co
     TC_REQUIRE((uintptr_t)table % t_esz == 0 && (uintptr_t)out % o_esz == 0 && (uintptr_t)tokens % id_bytes == 0,
                "tc_embedding_fwd: misaligned operand");
     if (pad_idx < 0) pad_idx = INT64_MIN;          // no padding id
-    // 16-byte stores where the rows allow them: 4 f32 or 8 bf16 values
+    // 16-byte stores, 4 f32 or 8 bf16 values; rows that start anywhere or end inside a piece take the loose form
     const int wide = out_dtype == TC_BF16 ? 8 : 4;
-    const bool vec = tc_rows_aligned(table, E, t_esz, wide) && tc_rows_aligned(out, E, o_esz, wide);
-    const int pieces = vec ? E / wide : E;
+    const bool loose = !(tc_rows_aligned(table, E, t_esz, wide) && tc_rows_aligned(out, E, o_esz, wide));
+    const int pieces = (E + wide - 1) / wide;
     int lanes_log2 = 0;
     while (lanes_log2 < 6 && (1 << lanes_log2) < pieces) ++lanes_log2;
     long blocks = ((M << lanes_log2) + 255) / 256;
     if (blocks > (1L << 20)) blocks = 1L << 20;    // a launch holds fewer than 2^32 threads; rows are walked with the grid's stride
     hipStream_t s = static_cast<hipStream_t>(stream);
     TcProfScope prof(TC_PROF_EMBED, s, (double)M * E * o_esz);
-#define TC_EMB(TT, TO, TID, V)                                                                              \
-    TC_LAUNCH((embedding_kernel<TT, TO, TID, V>), dim3((unsigned)blocks), dim3(256), 0, s,                  \
+#define TC_EMB(TT, TO, TID, V, L)                                                                           \
+    TC_LAUNCH((embedding_kernel<TT, TO, TID, V, L>), dim3((unsigned)blocks), dim3(256), 0, s,               \
               static_cast<const TID *>(tokens), static_cast<const TT *>(table), static_cast<TO *>(out), M, E, vocab, scale, \
               pad_idx, lanes_log2, bad)
-#define TC_EMB_ID(TT, TO, V) do { if (id_bytes == 4) TC_EMB(TT, TO, int32_t, V); else TC_EMB(TT, TO, int64_t, V); } while (0)
-#define TC_EMB_V(TT, TO, W) do { if (vec) TC_EMB_ID(TT, TO, W); else TC_EMB_ID(TT, TO, 1); } while (0)
+#define TC_EMB_ID(TT, TO, V, L) do { if (id_bytes == 4) TC_EMB(TT, TO, int32_t, V, L); else TC_EMB(TT, TO, int64_t, V, L); } while (0)
+#define TC_EMB_L(TT, TO, V) do { if (loose) TC_EMB_ID(TT, TO, V, true); else TC_EMB_ID(TT, TO, V, false); } while (0)
     if (table_dtype == TC_F32) {
-        if (out_dtype == TC_F32) TC_EMB_V(float, float, 4);
-        else TC_EMB_V(float, uint16_t, 8);
+        if (out_dtype == TC_F32) TC_EMB_L(float, float, 4);
+        else TC_EMB_L(float, uint16_t, 8);
     } else {
-        if (out_dtype == TC_F32) TC_EMB_V(uint16_t, float, 4);
-        else TC_EMB_V(uint16_t, uint16_t, 8);
+        if (out_dtype == TC_F32) TC_EMB_L(uint16_t, float, 4);
+        else TC_EMB_L(uint16_t, uint16_t, 8);
     }
-#undef TC_EMB_V
+#undef TC_EMB_L
 #undef TC_EMB_ID
 #undef TC_EMB
     TC_CHECK_LAUNCH("tc_embedding_fwd");
@@ -501,16 +503,16 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
     if (pad_idx < 0) pad_idx = INT64_MIN;
     char *ws = static_cast<char *>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const bool vec = tc_rows_aligned(dy, ld_dy, esz, 4) && tc_rows_aligned(d_table, E, 4, 4);
-    const unsigned slabs = (unsigned)((E + (vec ? 255 : 63)) / (vec ? 256 : 64));
+    const bool loose = !(tc_rows_aligned(dy, ld_dy, esz, VEC) && tc_rows_aligned(d_table, E, 4, VEC));
+    const unsigned slabs = (unsigned)((E + 64 * VEC - 1) / (64 * VEC));
 #define TC_EMB_T(KERNEL, GRID, BLOCK, P)                                                                                        \
     do {                                                                                                                        \
         if (dy_dtype == TC_F32) {                                                                                               \
-            if (vec) TC_LAUNCH((KERNEL(float, 4)), GRID, dim3(BLOCK), 0, s, P);                                                 \
-            else TC_LAUNCH((KERNEL(float, 1)), GRID, dim3(BLOCK), 0, s, P);                                                     \
+            if (loose) TC_LAUNCH((KERNEL(float, true)), GRID, dim3(BLOCK), 0, s, P);                                            \
+            else TC_LAUNCH((KERNEL(float, false)), GRID, dim3(BLOCK), 0, s, P);                                                 \
         } else {                                                                                                                \
-            if (vec) TC_LAUNCH((KERNEL(uint16_t, 4)), GRID, dim3(BLOCK), 0, s, P);                                              \
-            else TC_LAUNCH((KERNEL(uint16_t, 1)), GRID, dim3(BLOCK), 0, s, P);                                                  \
+            if (loose) TC_LAUNCH((KERNEL(uint16_t, true)), GRID, dim3(BLOCK), 0, s, P);                                         \
+            else TC_LAUNCH((KERNEL(uint16_t, false)), GRID, dim3(BLOCK), 0, s, P);                                              \
         }                                                                                                                       \
     } while (0)
     if (M <= kFew) {
@@ -519,8 +521,8 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
         f.M = (int)M; f.E = E; f.accumulate = accumulate; f.scale = scale;
         const long want = (vocab + 3) / 4, most = 8192 / slabs > 256 ? 8192 / slabs : 256;
         const dim3 grid((unsigned)(want < most ? want : most), slabs);
-#define TC_FEW4(T, V) few_positions_kernel<T, int32_t, V>
-#define TC_FEW8(T, V) few_positions_kernel<T, int64_t, V>
+#define TC_FEW4(T, L) few_positions_kernel<T, int32_t, L>
+#define TC_FEW8(T, L) few_positions_kernel<T, int64_t, L>
         if (id_bytes == 4) TC_EMB_T(TC_FEW4, grid, 256, f);
         else TC_EMB_T(TC_FEW8, grid, 256, f);
         TC_CHECK_LAUNCH("tc_embedding_bwd");
@@ -566,11 +568,11 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
     q.part_ld = w.part_ld;
     q.M = (int)M; q.E = E; q.spans = w.spans;
     q.accumulate = accumulate; q.vocab = (uint32_t)vocab; q.scale = scale;
-#define TC_SUM(T, V) segment_sum_kernel<T, V>
+#define TC_SUM(T, L) segment_sum_kernel<T, L>
     TC_EMB_T(TC_SUM, dim3((unsigned)w.spans, slabs), 64 * kSumWaves, q);
     if (w.spans > 1) {
-        if (vec) TC_LAUNCH(segment_join_kernel<4>, dim3((unsigned)(w.spans + 3) / 4, slabs), dim3(256), 0, s, q);
-        else TC_LAUNCH(segment_join_kernel<1>, dim3((unsigned)(w.spans + 3) / 4, slabs), dim3(256), 0, s, q);
+        if (loose) TC_LAUNCH(segment_join_kernel<true>, dim3((unsigned)(w.spans + 3) / 4, slabs), dim3(256), 0, s, q);
+        else TC_LAUNCH(segment_join_kernel<false>, dim3((unsigned)(w.spans + 3) / 4, slabs), dim3(256), 0, s, q);
     }
 #undef TC_SUM
 #undef TC_FEW8

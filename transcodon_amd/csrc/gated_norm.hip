@@ -7,13 +7,16 @@
 // and its backward pass.  norm(t) = (t - mean) * rstd, or t * rstd for root-mean-square norms (mean = 0).  The residual
 // stream and all arithmetic are f32; y, h and their gradients are f32 or bf16.
 //
-// A team of W waves owns a row at a time and keeps it in registers (W = 1 up to 1024 columns), so every operand is
-// read from memory once; deviations are summed after the mean is known.  The backward pass gives each team a run of
+// A team of W waves owns a row at a time and keeps it in registers, so every operand is read from memory once; deviations are
+// summed after the mean is known.  HBM bound: 65536 x 768 in bf16 with 64 gate rows 115 us forward (604 MB, 5.3 TB/s; a
+// large copy: 4.9) and 208 us backward (907 MB, 4.35 TB/s).  The backward pass gives each team a run of
 // neighbouring rows and keeps the column sums (gradients of the norms' vectors and of the gate) in registers; teams of
 // a workgroup are added in LDS, workgroups by a second kernel, always in the same order.
 #include "row_io.h"
 
 namespace {
+
+constexpr int VEC = 4;                       // neighbouring values of a row that a lane loads at a time
 
 template <int W>
 struct Team {                                // W waves that work on one row
@@ -41,8 +44,8 @@ struct Team {                                // W waves that work on one row
 };
 
 // mean and 1 / sqrt(variance + eps) of a row held as v[NC][VEC]
-template <int W, int NC, int VEC>
-__device__ __forceinline__ void row_stats(Team<W> &team, const float (&v)[NC][VEC], const bool (&in)[NC], int E, int rms, float eps,
+template <int W, int NC>
+__device__ __forceinline__ void row_stats(Team<W> &team, const float (&v)[NC][VEC], const int (&n)[NC], int E, int rms, float eps,
                                           float &mean, float &rstd) {
     mean = 0.f;
     if (!rms) {
@@ -56,12 +59,10 @@ __device__ __forceinline__ void row_stats(Team<W> &team, const float (&v)[NC][VE
     float q = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
-        if (in[c]) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float d = v[c][j] - mean;
-                q += d * d;
-            }
+        for (int j = 0; j < VEC; ++j) {
+            const float d = j < n[c] ? v[c][j] - mean : 0.f;
+            q += d * d;
         }
     rstd = rsqrtf(team.sum(q) / (float)E + eps);
 }
@@ -86,64 +87,88 @@ struct NormParams {
     int teams, rows_per_team, teams_per_group;
 };
 
-template <typename T, typename TG, int VEC, int W, int NC>
+template <typename T, typename TG, bool LOOSE, int W, int NC>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_kernel(const NormParams p) {
     __shared__ float red[2][2][W];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Team<W> team{red, W == 1 ? 0 : wave};
     constexpr int kTeams = W == 1 ? 4 : 1;
     const int col0 = ((W == 1 ? 0 : wave) * 64 + lane) * VEC;
-    bool in[NC];
+    int n[NC];                               // values of each piece that the row has
 #pragma unroll
-    for (int c = 0; c < NC; ++c) in[c] = col0 + c * 64 * W * VEC < p.E;
-    for (long row = (long)blockIdx.x * kTeams + (W == 1 ? wave : 0); row < p.M; row += (long)gridDim.x * kTeams) {
+    for (int c = 0; c < NC; ++c) {
+        const int left = p.E - (col0 + c * 64 * W * VEC);
+        n[c] = LOOSE ? max(0, min(VEC, left)) : left > 0 ? VEC : 0;
+    }
+    // Two teams of 16 waves fill a CU and meet at barriers: they ask for their next row before they work on this one (4096 x
+    // 8192 bf16: 139 -> 117 us).  Smaller teams find others to hide their loads behind (8192 x 4096: 90 us, asking ahead 93).
+    constexpr bool kAhead = W == 16;
+    struct Row {
+        typename TcRaw<T, VEC>::type y[NC];
+        typename TcRaw<float, VEC>::type x[NC];
+    } next;
+    auto request = [&](long row) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = col0 + c * 64 * W * VEC;
+            if (n[c] == 0) continue;
+            next.y[c] = tc_raw_load<T, VEC, LOOSE>(static_cast<const T *>(p.y) + row * p.ldy + col, n[c]);
+            next.x[c] = tc_raw_load<float, VEC, LOOSE>(p.x + row * p.ldx + col, n[c]);
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        next.y[c] = typename TcRaw<T, VEC>::type{};
+        next.x[c] = typename TcRaw<float, VEC>::type{};
+    }
+    const long step = (long)gridDim.x * kTeams;
+    long row = (long)blockIdx.x * kTeams + (W == 1 ? wave : 0);
+    if (kAhead && row < p.M) request(row);
+    for (; row < p.M; row += step) {
+        if (!kAhead) request(row);
         float yv[NC][VEC], xv[NC][VEC];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = col0 + c * 64 * W * VEC;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) yv[c][j] = xv[c][j] = 0.f;
-            if (in[c]) {
-                tc_load_row<T, VEC>(static_cast<const T *>(p.y) + row * p.ldy + col, yv[c]);
-                tc_load_row<float, VEC>(p.x + row * p.ldx + col, xv[c]);
-            }
+            tc_raw_widen<T, VEC>(next.y[c], yv[c]);
+            tc_raw_widen<float, VEC>(next.x[c], xv[c]);
         }
+        if (kAhead && row + step < p.M) request(row + step);
         float mean1, rstd1;
-        row_stats<W, NC, VEC>(team, yv, in, p.E, p.rms, p.eps1, mean1, rstd1);
-        const long gate_row = (row / p.rows_per_gate) * p.E;
+        row_stats<W, NC>(team, yv, n, p.E, p.rms, p.eps1, mean1, rstd1);
+        const long gate_row = (long)((unsigned)row / (unsigned)p.rows_per_gate) * p.E;      // rows are below 2^31
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int col = col0 + c * 64 * W * VEC;
-            if (!in[c]) continue;
+            if (n[c] == 0) continue;
             float g[VEC], b[VEC], gt[VEC];
-            tc_load_row<float, VEC>(p.g1 + col, g);
-            if (p.b1) tc_load_row<float, VEC>(p.b1 + col, b);
-            if (p.gate) tc_load_row<TG, VEC>(static_cast<const TG *>(p.gate) + gate_row + col, gt);
+            tc_load_row<float, VEC, LOOSE>(p.g1 + col, g, n[c]);
+            if (p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + col, b, n[c]);
+            if (p.gate) tc_load_row<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + gate_row + col, gt, n[c]);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                float n = (yv[c][j] - mean1) * rstd1 * g[j];
-                if (p.b1) n += b[j];
-                if (p.gate) n *= gt[j];
-                xv[c][j] = p.res_scale * xv[c][j] + n;
+                float t = (yv[c][j] - mean1) * rstd1 * g[j];
+                if (p.b1) t += b[j];
+                if (p.gate) t *= gt[j];
+                xv[c][j] = p.res_scale * xv[c][j] + t;
             }
-            tc_store_row<float, VEC>(p.x_out + row * p.E + col, xv[c]);
+            tc_store_row<float, VEC, LOOSE>(p.x_out + row * p.E + col, xv[c], n[c]);
         }
         float mean2 = 0.f, rstd2 = 0.f;
         if (p.g2) {
-            row_stats<W, NC, VEC>(team, xv, in, p.E, p.rms, p.eps2, mean2, rstd2);
+            row_stats<W, NC>(team, xv, n, p.E, p.rms, p.eps2, mean2, rstd2);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int col = col0 + c * 64 * W * VEC;
-                if (!in[c]) continue;
+                if (n[c] == 0) continue;
                 float g[VEC], b[VEC];
-                tc_load_row<float, VEC>(p.g2 + col, g);
-                if (p.b2) tc_load_row<float, VEC>(p.b2 + col, b);
+                tc_load_row<float, VEC, LOOSE>(p.g2 + col, g, n[c]);
+                if (p.b2) tc_load_row<float, VEC, LOOSE>(p.b2 + col, b, n[c]);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     xv[c][j] = (xv[c][j] - mean2) * rstd2 * g[j];
                     if (p.b2) xv[c][j] += b[j];
                 }
-                tc_store_row<T, VEC>(static_cast<T *>(p.h) + row * p.E + col, xv[c]);
+                tc_store_row<T, VEC, LOOSE>(static_cast<T *>(p.h) + row * p.E + col, xv[c], n[c]);
             }
         }
         if (p.stats && col0 == 0) *reinterpret_cast<f32x4 *>(p.stats + row * 4) = f32x4{mean1, rstd1, mean2, rstd2};
@@ -155,18 +180,21 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_kernel(const
 //   y^ = (y - mean1) rstd1        dn = D o gate     dy = rstd1 (q - mean(q) - y^ mean(q y^)),  q = dn o g1
 //   dx = res_scale D    d_gate = sum D o n    d_g1 = sum dn o y^   d_b1 = sum dn   d_g2 = sum dh o x^   d_b2 = sum dh
 // (root-mean-square norms: without the mean(p), mean(q) terms).
-template <typename T, typename TG, int VEC, int W, int NC>
+template <typename T, typename TG, bool LOOSE, int W, int NC>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(const NormParams p) {
-    extern __shared__ float sums[];          // [4][E] of the workgroup (W == 1)
+    extern __shared__ float sums[];          // [team][E] (W == 1)
     __shared__ float red[2][2][W];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Team<W> team{red, W == 1 ? 0 : wave};
     constexpr int kTeams = W == 1 ? 4 : 1;   // teams of a workgroup
     const int t = blockIdx.x * kTeams + (W == 1 ? wave : 0);
     const int col0 = ((W == 1 ? 0 : wave) * 64 + lane) * VEC;
-    bool in[NC];
+    int n[NC];                               // values of each piece that the row has
 #pragma unroll
-    for (int c = 0; c < NC; ++c) in[c] = col0 + c * 64 * W * VEC < p.E;
+    for (int c = 0; c < NC; ++c) {
+        const int left = p.E - (col0 + c * 64 * W * VEC);
+        n[c] = LOOSE ? max(0, min(VEC, left)) : left > 0 ? VEC : 0;
+    }
     float acc[4][NC][VEC], dgt[NC][VEC];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -187,31 +215,55 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
     }
     if (t >= p.teams) begin = end = 0;
     const float inv_e = 1.0f / (float)p.E;
-    for (long row = begin; row < end; ++row) {
-        float yv[NC][VEC], xv[NC][VEC], dh[NC][VEC], d[NC][VEC];
+    // A row's operands as they were loaded.  The next row is requested before this one is worked on: three dependent row
+    // reductions per row leave a wave idle otherwise, and the registers allow only two or three waves a SIMD.  (Not with
+    // 16 waves, which leave 128 registers each, or 16 values a lane: there the second row would not fit.)
+    constexpr bool kAhead = NC * VEC <= 12 && W < 16;
+    struct Row {
+        typename TcRaw<T, VEC>::type y[NC], dh[NC];
+        typename TcRaw<float, VEC>::type x[NC], d[NC];
+        f32x4 st;
+    } next;
+    auto request = [&](long row) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int col = col0 + c * 64 * W * VEC;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) yv[c][j] = xv[c][j] = dh[c][j] = d[c][j] = 0.f;
-            if (in[c]) {
-                tc_load_row<T, VEC>(static_cast<const T *>(p.y) + row * p.ldy + col, yv[c]);
-                if (p.g2) {
-                    tc_load_row<float, VEC>(p.x + row * p.ldx + col, xv[c]);
-                    tc_load_row<T, VEC>(static_cast<const T *>(p.dh) + row * p.ld_dh + col, dh[c]);
-                }
-                if (p.dx_out) tc_load_row<float, VEC>(p.dx_out + row * p.ld_dxo + col, d[c]);
+            if (n[c] == 0) continue;
+            next.y[c] = tc_raw_load<T, VEC, LOOSE>(static_cast<const T *>(p.y) + row * p.ldy + col, n[c]);
+            if (p.g2) {
+                next.x[c] = tc_raw_load<float, VEC, LOOSE>(p.x + row * p.ldx + col, n[c]);
+                next.dh[c] = tc_raw_load<T, VEC, LOOSE>(static_cast<const T *>(p.dh) + row * p.ld_dh + col, n[c]);
             }
+            if (p.dx_out) next.d[c] = tc_raw_load<float, VEC, LOOSE>(p.dx_out + row * p.ld_dxo + col, n[c]);
         }
-        const f32x4 st = *reinterpret_cast<const f32x4 *>(p.stats + row * 4);
+        next.st = *reinterpret_cast<const f32x4 *>(p.stats + row * 4);
+    };
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        next.y[c] = next.dh[c] = typename TcRaw<T, VEC>::type{};
+        next.x[c] = next.d[c] = typename TcRaw<float, VEC>::type{};
+    }
+    if (kAhead && begin < end) request(begin);
+    for (long row = begin; row < end; ++row) {
+        if (!kAhead) request(row);
+        float yv[NC][VEC], xv[NC][VEC], dh[NC][VEC], d[NC][VEC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            tc_raw_widen<T, VEC>(next.y[c], yv[c]);
+            tc_raw_widen<float, VEC>(next.x[c], xv[c]);
+            tc_raw_widen<T, VEC>(next.dh[c], dh[c]);
+            tc_raw_widen<float, VEC>(next.d[c], d[c]);
+        }
+        const f32x4 st = next.st;
+        if (kAhead && row + 1 < end) request(row + 1);
         if (p.g2) {
             float s1 = 0.f, s2 = 0.f;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int col = col0 + c * 64 * W * VEC;
-                if (!in[c]) continue;
+                if (n[c] == 0) continue;
                 float g[VEC];
-                tc_load_row<float, VEC>(p.g2 + col, g);
+                tc_load_row<float, VEC, LOOSE>(p.g2 + col, g, n[c]);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     const float xh = (xv[c][j] - st[2]) * st[3];
@@ -231,24 +283,24 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) d[c][j] += st[3] * (dh[c][j] - m1 - xv[c][j] * m2);
         }
-        const long gate_row = (row / p.rows_per_gate) * p.E;
+        const long gate_row = (long)((unsigned)row / (unsigned)p.rows_per_gate) * p.E;      // rows are below 2^31
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int col = col0 + c * 64 * W * VEC;
-            if (!in[c]) continue;
+            if (n[c] == 0) continue;
             float g[VEC], b[VEC], gt[VEC], o[VEC];
-            tc_load_row<float, VEC>(p.g1 + col, g);
-            if (p.gate) tc_load_row<TG, VEC>(static_cast<const TG *>(p.gate) + gate_row + col, gt);
-            if (p.gate && p.b1) tc_load_row<float, VEC>(p.b1 + col, b);
+            tc_load_row<float, VEC, LOOSE>(p.g1 + col, g, n[c]);
+            if (p.gate) tc_load_row<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + gate_row + col, gt, n[c]);
+            if (p.gate && p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + col, b, n[c]);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 const float yh = (yv[c][j] - st[0]) * st[1];
                 float dn = d[c][j];
                 if (p.gate) {
-                    float n = yh * g[j];
-                    if (p.b1) n += b[j];
-                    dgt[c][j] += dn * n;
+                    float t = yh * g[j];
+                    if (p.b1) t += b[j];
+                    dgt[c][j] += dn * t;
                     dn *= gt[j];
                 }
                 acc[0][c][j] += dn * yh;
@@ -260,33 +312,33 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
                 yv[c][j] = yh;
                 d[c][j] = q;
             }
-            tc_store_row<float, VEC>(p.dx + row * p.E + col, o);
+            tc_store_row<float, VEC, LOOSE>(p.dx + row * p.E + col, o, n[c]);
         }
         team.sum2(s1, s2);
         const float m1 = p.rms ? 0.f : s1 * inv_e, m2 = s2 * inv_e;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int col = col0 + c * 64 * W * VEC;
-            if (!in[c]) continue;
+            if (n[c] == 0) continue;
             float o[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) o[j] = st[1] * (d[c][j] - m1 - yv[c][j] * m2);
-            tc_store_row<T, VEC>(static_cast<T *>(p.dy) + row * p.E + col, o);
+            tc_store_row<T, VEC, LOOSE>(static_cast<T *>(p.dy) + row * p.E + col, o, n[c]);
         }
         // the team's last row of a gate group: the group's gradient, or this team's part of it
-        if (p.gate && p.teams_per_group == 0 && (row + 1) % p.rows_per_gate == 0) {
+        if (p.gate && p.teams_per_group == 0 && ((unsigned)row + 1) % (unsigned)p.rows_per_gate == 0) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int col = col0 + c * 64 * W * VEC;
-                if (!in[c]) continue;
+                if (n[c] == 0) continue;
                 float *to = p.d_gate + gate_row + col;
                 if (p.accumulate & 16) {
                     float old[VEC];
-                    tc_load_row<float, VEC>(to, old);
+                    tc_load_row<float, VEC, LOOSE>(to, old, n[c]);
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) dgt[c][j] += old[j];
                 }
-                tc_store_row<float, VEC>(to, dgt[c]);
+                tc_store_row<float, VEC, LOOSE>(to, dgt[c], n[c]);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) dgt[c][j] = 0.f;
             }
@@ -298,37 +350,31 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int col = col0 + c * 64 * W * VEC;
-            if (in[c])
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) to[col + j] = dgt[c][j];
+            if (n[c] > 0) tc_store_row<float, VEC, LOOSE>(to + col, dgt[c], n[c]);
         }
     }
     float *to = p.ws + (long)blockIdx.x * 4 * p.E;
     if constexpr (W == 1) {
-        for (int w = 0; w < kTeams; ++w) {
-            if (wave == w) {
 #pragma unroll
-                for (int v = 0; v < 4; ++v)
+        for (int v = 0; v < 4; ++v) {
 #pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        const int col = col0 + c * 64 * VEC;
-                        if (in[c])
+            for (int c = 0; c < NC; ++c) {
+                const int col = col0 + c * 64 * VEC;
 #pragma unroll
-                            for (int j = 0; j < VEC; ++j) sums[v * p.E + col + j] = w == 0 ? acc[v][c][j] : sums[v * p.E + col + j] + acc[v][c][j];
-                    }
+                for (int j = 0; j < VEC; ++j)
+                    if (j < n[c]) sums[wave * p.E + col + j] = acc[v][c][j];
             }
             __syncthreads();
+            for (int i = threadIdx.x; i < p.E; i += 256) to[v * p.E + i] = (sums[i] + sums[p.E + i]) + (sums[2 * p.E + i] + sums[3 * p.E + i]);
+            __syncthreads();
         }
-        for (int i = threadIdx.x; i < 4 * p.E; i += 256) to[i] = sums[i];
     } else {
 #pragma unroll
         for (int v = 0; v < 4; ++v)
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int col = col0 + c * 64 * W * VEC;
-                if (in[c])
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) to[(long)v * p.E + col + j] = acc[v][c][j];
+                if (n[c] > 0) tc_store_row<float, VEC, LOOSE>(to + (long)v * p.E + col, acc[v][c], n[c]);
             }
     }
 }
@@ -360,25 +406,38 @@ __global__ __launch_bounds__(1024) void gated_norm_join_kernel(const NormParams 
     }
 }
 
-// Waves per row and values per lane: one wave up to 1024 columns, four up to 4096, eight up to 8192.
-int waves_per_row(int E) { return E <= 1024 ? 1 : E <= 4096 ? 4 : 8; }
+// How a row is laid over lanes: W waves a row, NC loads of VEC values a lane and operand.  Rows whose width or addresses do
+// not allow aligned loads take the LOOSE form: unaligned ones, and the values of a row's end one by one.
+// One wave a row needs no barrier and is the faster form for many rows (65536 x 768 bf16: forward 115 against 150 us with
+// four waves, backward 208 against 228; 8192 rows: forward 16.5 / 19.6, backward 33.0 / 32.4).  With few rows, or rows of narrow loads,
+// it leaves the chip idle: 4101 x 770 f32 backward 47 us with one wave, 29 with four.
+constexpr long kManyRows = 8192;
+struct Shape {
+    int W, nc;
+};
+Shape row_shape(long M, int E) {
+    const int W = E <= 1024 && M >= kManyRows ? 1 : E <= 2048 ? 4 : E <= 4096 ? 8 : 16;
+    return Shape{W, (E + 64 * VEC * W - 1) / (64 * VEC * W)};
+}
 
 struct BwdPlan {
     int teams, rows_per_team, teams_per_group, workgroups;
     size_t bytes;
 };
-BwdPlan bwd_plan(int M, int E, int G) {
+BwdPlan bwd_plan(int M, int E, int G, int W) {
     BwdPlan w{};
-    const int W = waves_per_row(E), per_wg = W == 1 ? 4 : 1;
-    const int want = 2048 / W * (W == 1 ? 1 : 2);
-    const int rows = (M + want - 1) / want;
+    const int per_wg = W == 1 ? 4 : 1;
+    // Teams: enough to fill the chip once.  One wave a row: 2048 waves are 210 us at 65536 x 768 bf16 (1024: 245, 3072: 252, 4096: 215).
+    // Four waves: 1024 workgroups are 28.7 us at 4101 x 770 f32 (512: 29.5, 2048: 32.8: every workgroup leaves 4 E sums).
+    const int want = W == 1 ? 2048 : 4096 / W;
+    const int rows = (int)(((long)M + want - 1) / want);
     const int group = G > 0 ? M / G : 0;
     if (G == 0 || group <= rows) {
         w.rows_per_team = G == 0 ? rows : rows / group * group;
-        w.teams = (M + w.rows_per_team - 1) / w.rows_per_team;
+        w.teams = (int)(((long)M + w.rows_per_team - 1) / w.rows_per_team);
     } else {
-        w.teams_per_group = (group + rows - 1) / rows;
-        w.rows_per_team = (group + w.teams_per_group - 1) / w.teams_per_group;
+        w.teams_per_group = (int)(((long)group + rows - 1) / rows);
+        w.rows_per_team = (int)(((long)group + w.teams_per_group - 1) / w.teams_per_group);
         w.teams = G * w.teams_per_group;
     }
     w.workgroups = (w.teams + per_wg - 1) / per_wg;
@@ -398,25 +457,29 @@ int check_common(const char *who, int dtype, int gate_dtype, const void *gate, l
 
 }  // namespace
 
-#define TC_GN_NC(K, T, TG, W)                                                                   \
+#define TC_GN_W(K, T, TG, LOOSE)                                                                \
     do {                                                                                        \
-        if (!vec) TC_GN(K, T, TG, 1, W, 16);                                                    \
-        else if (E <= 64 * 4 * W) TC_GN(K, T, TG, 4, W, 1);                                     \
-        else if (E <= 64 * 8 * W) TC_GN(K, T, TG, 4, W, 2);                                     \
-        else if (E <= 64 * 12 * W) TC_GN(K, T, TG, 4, W, 3);                                    \
-        else TC_GN(K, T, TG, 4, W, 4);                                                          \
+        switch (sh.W * 10 + sh.nc) {                                                            \
+            case 11: TC_GN(K, T, TG, LOOSE, 1, 1); break;                                       \
+            case 12: TC_GN(K, T, TG, LOOSE, 1, 2); break;                                       \
+            case 13: TC_GN(K, T, TG, LOOSE, 1, 3); break;                                       \
+            case 14: TC_GN(K, T, TG, LOOSE, 1, 4); break;                                       \
+            case 41: TC_GN(K, T, TG, LOOSE, 4, 1); break;                                       \
+            case 42: TC_GN(K, T, TG, LOOSE, 4, 2); break;                                       \
+            case 82: TC_GN(K, T, TG, LOOSE, 8, 2); break;                                       \
+            default: TC_GN(K, T, TG, LOOSE, 16, 2); break;                                      \
+        }                                                                                       \
     } while (0)
-#define TC_GN_W(K, T, TG)                                                                       \
+#define TC_GN_L(K, T, TG)                                                                       \
     do {                                                                                        \
-        if (W == 1) TC_GN_NC(K, T, TG, 1);                                                      \
-        else if (W == 4) TC_GN_NC(K, T, TG, 4);                                                 \
-        else TC_GN_NC(K, T, TG, 8);                                                             \
+        if (loose) TC_GN_W(K, T, TG, true);                                                     \
+        else TC_GN_W(K, T, TG, false);                                                          \
     } while (0)
 #define TC_GN_T(K)                                                                              \
     do {                                                                                        \
-        if (dtype == TC_F32) TC_GN_W(K, float, float);                                          \
-        else if (gate_dtype == TC_F32) TC_GN_W(K, uint16_t, float);                             \
-        else TC_GN_W(K, uint16_t, uint16_t);                                                    \
+        if (dtype == TC_F32) TC_GN_L(K, float, float);                                          \
+        else if (gate_dtype == TC_F32) TC_GN_L(K, uint16_t, float);                             \
+        else TC_GN_L(K, uint16_t, uint16_t);                                                    \
     } while (0)
 
 extern "C" int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, const float *x, long ldx, const float *post_gamma,
@@ -443,16 +506,18 @@ extern "C" int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, co
     p.rows_per_gate = G > 0 ? (int)(M / G) : (int)M;
     p.res_scale = res_scale; p.eps1 = post_eps; p.eps2 = pre_eps;
     const int g_esz = gate_dtype == TC_BF16 ? 2 : 4;
-    const bool vec = tc_rows_aligned(y, ldy, esz, 4) && tc_rows_aligned(x, ldx, 4, 4) && tc_rows_aligned(gate, E, g_esz, 4) &&
-                     tc_rows_aligned(h, E, esz, 4) && tc_aligned16(x_out) && tc_aligned16(post_gamma) && tc_aligned16(post_beta) &&
-                     tc_aligned16(pre_gamma) && tc_aligned16(pre_beta);
-    const int W = waves_per_row(E), per_wg = W == 1 ? 4 : 1;
+    const bool loose = !(tc_rows_aligned(y, ldy, esz, VEC) && tc_rows_aligned(x, ldx, 4, VEC) && tc_rows_aligned(gate, E, g_esz, VEC) &&
+               tc_rows_aligned(h, E, esz, VEC) && tc_rows_aligned(x_out, E, 4, VEC) && tc_rows_aligned(post_gamma, 0, 4, VEC) &&
+               tc_rows_aligned(post_beta, 0, 4, VEC) && tc_rows_aligned(pre_gamma, 0, 4, VEC) && tc_rows_aligned(pre_beta, 0, 4, VEC));
+    const Shape sh = row_shape(M, E);
+    const int per_wg = sh.W == 1 ? 4 : 1;
     long blocks = (M + per_wg - 1) / per_wg;
-    const long most = 1L << 22;                    // a launch holds fewer than 2^32 threads; rows are walked with the grid's stride
+    // rows are walked with the grid's stride: a launch holds fewer than 2^32 threads, and teams that ask ahead fill the chip once
+    const long most = sh.W == 16 ? 512 : 1L << 21;
     if (blocks > most) blocks = most;
     hipStream_t s = static_cast<hipStream_t>(stream);
     TcProfScope prof(TC_PROF_LAYERNORM, s, (double)M * E * (2 * esz + 8));
-#define TC_GN(K, T, TG, V, WW, N) TC_LAUNCH((K<T, TG, V, WW, N>), dim3((unsigned)blocks), dim3(WW == 1 ? 256 : 64 * WW), 0, s, p)
+#define TC_GN(K, T, TG, L, WW, N) TC_LAUNCH((K<T, TG, L, WW, N>), dim3((unsigned)blocks), dim3(WW == 1 ? 256 : 64 * WW), 0, s, p)
     TC_GN_T(gated_norm_kernel);
 #undef TC_GN
     TC_CHECK_LAUNCH("tc_gated_residual_norm_fwd");
@@ -461,7 +526,13 @@ extern "C" int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, co
 
 extern "C" size_t tc_gated_residual_norm_bwd_workspace_bytes(long M, int E, int G) {
     if (M <= 0 || M > 0x7fffffffL || E <= 0 || E > 8192 || G < 0 || (G > 0 && M % G != 0)) return 0;
-    return bwd_plan((int)M, E, G).bytes;
+    // which layout a call takes depends on its addresses too: enough for each
+    size_t most = 16;
+    for (int W : {1, 4, 8, 16}) {
+        const size_t n = bwd_plan((int)M, E, G, W).bytes;
+        most = n > most ? n : most;
+    }
+    return most;
 }
 
 extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh, const float *dx_out, long ld_dxo, const void *y,
@@ -486,11 +557,18 @@ extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh,
                     (uintptr_t)pre_gamma | (uintptr_t)d_post_gamma | (uintptr_t)d_post_beta | (uintptr_t)d_gate |
                     (uintptr_t)d_pre_gamma | (uintptr_t)d_pre_beta) % 4 == 0,
                "tc_gated_residual_norm_bwd: misaligned operand (stats and workspace: 16 bytes)");
-    const BwdPlan w = bwd_plan((int)M, E, G);
-    if (workspace_bytes < w.bytes) {
-        tc_set_error("tc_gated_residual_norm_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, w.bytes);
+    const size_t need = tc_gated_residual_norm_bwd_workspace_bytes(M, E, G);
+    if (workspace_bytes < need) {
+        tc_set_error("tc_gated_residual_norm_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
         return TC_ENOSPC;
     }
+    const int g_esz = gate_dtype == TC_BF16 ? 2 : 4;
+    const bool loose = !(tc_rows_aligned(y, ldy, esz, VEC) && tc_rows_aligned(x_out, ldx, 4, VEC) && tc_rows_aligned(gate, E, g_esz, VEC) &&
+               (!dh || tc_rows_aligned(dh, ld_dh, esz, VEC)) && (!dx_out || tc_rows_aligned(dx_out, ld_dxo, 4, VEC)) &&
+               tc_rows_aligned(dy, E, esz, VEC) && tc_rows_aligned(dx, E, 4, VEC) && tc_rows_aligned(d_gate, E, 4, VEC) &&
+               tc_rows_aligned(post_gamma, 0, 4, VEC) && tc_rows_aligned(post_beta, 0, 4, VEC) && tc_rows_aligned(pre_gamma, 0, 4, VEC));
+    const Shape sh = row_shape(M, E);
+    const BwdPlan w = bwd_plan((int)M, E, G, sh.W);
     NormParams p{};
     p.y = y; p.x = x_out; p.gate = gate; p.dh = dh; p.dx_out = dx_out;
     p.stats = const_cast<float *>(stats);
@@ -504,16 +582,10 @@ extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh,
     p.rows_per_gate = G > 0 ? (int)(M / G) : (int)M;
     p.res_scale = res_scale;
     p.teams = w.teams; p.rows_per_team = w.rows_per_team; p.teams_per_group = w.teams_per_group;
-    const int g_esz = gate_dtype == TC_BF16 ? 2 : 4;
-    const bool vec = tc_rows_aligned(y, ldy, esz, 4) && tc_rows_aligned(x_out, ldx, 4, 4) && tc_rows_aligned(gate, E, g_esz, 4) &&
-                     (!dh || tc_rows_aligned(dh, ld_dh, esz, 4)) && (!dx_out || tc_rows_aligned(dx_out, ld_dxo, 4, 4)) &&
-                     tc_rows_aligned(dy, E, esz, 4) && tc_aligned16(dx) && tc_aligned16(d_gate) && tc_aligned16(post_gamma) &&
-                     tc_aligned16(post_beta) && tc_aligned16(pre_gamma);
-    const int W = waves_per_row(E);
     hipStream_t s = static_cast<hipStream_t>(stream);
     TcProfScope prof(TC_PROF_LAYERNORM, s, (double)M * E * (3 * esz + 12));
-#define TC_GN(K, T, TG, V, WW, N)                                                                                         \
-    TC_LAUNCH((K<T, TG, V, WW, N>), dim3((unsigned)w.workgroups), dim3(WW == 1 ? 256 : 64 * WW), WW == 1 ? 16 * (size_t)E : 0, s, p)
+#define TC_GN(K, T, TG, L, WW, N)                                                                                         \
+    TC_LAUNCH((K<T, TG, L, WW, N>), dim3((unsigned)w.workgroups), dim3(WW == 1 ? 256 : 64 * WW), WW == 1 ? 16 * (size_t)E : 0, s, p)
     TC_GN_T(gated_norm_bwd_kernel);
 #undef TC_GN
     const int groups = w.teams_per_group > 0 ? G : 0;

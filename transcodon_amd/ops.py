@@ -327,17 +327,18 @@ def colsum(x, want_bf16_copy=False, out=None):
 # ---- operators of a training block ---------------------------------------------------------------
 def _same_device(*tensors):
     """The common device of GPU tensors (None entries skipped); raises otherwise."""
-    dev = None
+    first, index = None, -1
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()
+        if i < 0:
             raise _lib.HipLibraryError("transcodon_amd kernels need tensors on the GPU (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return dev
+        if first is None:
+            first, index = t, i
+        elif i != index:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+    return first.device
 
 
 # handle of a device's current stream without a Stream object around it (2 us of a call's 7)
@@ -358,16 +359,18 @@ def _call(name, dev, *args):
 
 def _rows(t, name):
     """Row stride of a 2-d tensor whose columns are neighbours in memory."""
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
-        raise ValueError(f"{name} must be 2-d with unit column stride and rows that do not overlap")
-    return max(t.stride(0), t.shape[1])
+    if t.dim() == 2:
+        (M, E), (ld, step) = t.shape, t.stride()
+        if (step == 1 or E <= 1) and (ld >= E or M <= 1):
+            return ld if ld > E else E
+    raise ValueError(f"{name} must be 2-d with unit column stride and rows that do not overlap")
 
 
 def _dense(t, name, shape=None, dtype=None):
     """Checks a dense operand: its shape and element type where they are given."""
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} has type {t.dtype}, expected {dtype}")
@@ -505,15 +508,19 @@ def gated_residual_norm_bwd(dh, dx_out, y, x_out, stats, post_gamma, post_beta=N
     dy = torch.empty(M, E, dtype=y.dtype, device=dev)
     dx = torch.empty(M, E, dtype=torch.float32, device=dev)
     vectors = (post_gamma, post_beta, gate, pre_gamma, pre_beta)
+    empty = torch.empty if M and E else torch.zeros
+    # one allocation for the gradients of length E
+    fresh = iter(empty(4, E, dtype=torch.float32, device=dev).unbind(0))
     got, accumulate = [], 0
-    for v, given, bit in zip(vectors, into or (None,) * 5, (1, 2, 16, 4, 8)):
+    for i, v in enumerate(vectors):
+        given = into[i] if into else None
         if given is not None:
             if v is None:
                 raise ValueError("into has a buffer for a vector that is not there")
             _dense(given, "buffer in into", v.shape, torch.float32)
-            accumulate |= bit
+            accumulate |= (1, 2, 16, 4, 8)[i]
         elif v is not None:
-            given = (torch.empty if M and E else torch.zeros)(v.shape, dtype=torch.float32, device=dev)
+            given = empty(v.shape, dtype=torch.float32, device=dev) if i == 2 else next(fresh)
         got.append(given)
     if M and E:
         need = _lib.load().tc_gated_residual_norm_bwd_workspace_bytes(M, E, G)
