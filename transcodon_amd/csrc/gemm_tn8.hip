@@ -415,7 +415,10 @@ __global__ __launch_bounds__(512) void gemm_tn8_256_kernel(const Tn8Params p) {
             const int i = i0 + (a >> 2) * 128 + wr * 64 + (a & 3) * 16 + 4 * tg;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (i + r < p.N && j < p.K) out[(long)(i + r) * p.K + j] = acc[a][b][r];
+                if (i + r < p.N && j < p.K) {
+                    float *to = out + (long)(i + r) * p.K + j;
+                    *to = p.accumulate ? *to + acc[a][b][r] : acc[a][b][r];
+                }
         }
 }
 
@@ -428,27 +431,38 @@ struct Tn8Plan {
     bool big;                // 256 x 256 tiles over the whole stages, the rows behind them by the small kernel
     int splits, slabs;
 };
+// Which kernel and how many row splits: the least estimated time over both kernels and 1 .. 64 splits, in nanoseconds.
+// A stage takes a large tile 1.9 us on a full chip (220 us at 65536 x 2304 x 768: 114 stages), a small one 1 us while
+// there is one workgroup per CU and 0.6 us more for each further one; a part of the sum costs its slab written and read at
+// 6.5 TB/s, and more than one the summing launch.  Measured on either side of the rule: 262 x 768 x 768 in one part 10.0 us, in
+// five 14.7; 1024 x 768 x 768 in three 16.2, in sixteen 26.6; 65536 x 256 x 512 in 64 parts 55 us, in four 276.
 Tn8Plan tn8_plan(long M, long ld_dy, int N, int K) {
-    Tn8Plan w{};
+    Tn8Plan best{};
+    long least = -1;
     const long nk = (M + KT - 1) / KT, whole = M / KT;
-    const long tiles = (long)((N + 255) / 256) * ((K + 255) / 256);
-    // large tiles where they fill the chip once with at least two stages each and are not mostly padding
-    long s = 256 / tiles;
-    s = s < 1 ? 1 : s > 64 ? 64 : s;
-    const long rows = (whole / s + 4) * KT;        // of a split, and the stages loaded ahead
-    w.big = tiles * s >= 192 && whole >= 2 * s && tiles * 65536 <= (long)N * K * 3 / 2 && rows * ld_dy * 2 < (1L << 32) &&
-            rows * K < (1L << 32);
-    if (w.big) {
-        w.splits = (int)s;
-        w.slabs = w.splits + (M % KT != 0);
-        return w;
+    const long large = (long)((N + 255) / 256) * ((K + 255) / 256), small = (long)((N + 127) / 128) * ((K + 127) / 128);
+    auto parts = [&](long slabs) { return slabs > 1 ? 4000 + slabs * N * K * 8 / 6500 : 0; };
+    for (long s = 1; s <= 64; ++s) {
+        if (s <= nk) {
+            const long wgs = small * s;
+            const long ns = 2000 + (nk + s - 1) / s * (400 + 600 * (wgs > 256 ? wgs : 256) / 256) + parts(s);
+            if (least < 0 || ns < least) {
+                least = ns;
+                best = Tn8Plan{false, (int)s, (int)s};
+            }
+        }
+        // offsets inside a split, with the stages loaded ahead, are 32 bits
+        const long rows = (whole / s + 4) * KT;
+        if (whole >= 2 * s && rows * ld_dy * 2 < (1L << 32) && rows * K < (1L << 32)) {
+            const int rest = M % KT != 0;          // the rows behind the whole stages: one more part and launch
+            const long ns = 3000 + (whole + s - 1) / s * 1900 * ((large * s + 255) / 256) + 5000 * rest + parts(s + rest);
+            if (ns < least) {
+                least = ns;
+                best = Tn8Plan{true, (int)s, (int)s + rest};
+            }
+        }
     }
-    // about four workgroups per CU, no more than there are stages
-    const long small = (long)((N + 127) / 128) * ((K + 127) / 128);
-    s = 1024 / small;
-    s = s < 1 ? 1 : s > 64 ? 64 : s;
-    w.splits = w.slabs = (int)(s < nk ? s : nk);
-    return w;
+    return best;
 }
 
 }  // namespace
@@ -482,6 +496,7 @@ extern "C" int tc_gemm_tn_act8(const void *dy, long ld_dy, const void *codes, co
     p.splits = w.splits;
     p.out = w.slabs > 1 ? static_cast<float *>(workspace) : dW;
     p.slab_elems = (long)N * K;
+    p.accumulate = w.slabs > 1 ? 0 : accumulate;
     hipStream_t s = static_cast<hipStream_t>(stream);
     static_assert(LDS_BYTES <= 64 * 1024, "no attribute needed");
     const dim3 small_grid((unsigned)(((N + 127) / 128) * ((K + 127) / 128)), (unsigned)w.splits);
@@ -506,6 +521,7 @@ extern "C" int tc_gemm_tn_act8(const void *dy, long ld_dy, const void *codes, co
         if (M % KT != 0) {                         // the last rows: a part of their own
             const long done = M / KT * KT;
             Tn8Params t = p;
+            t.accumulate = 0;
             t.dy += done * p.ld_bytes;
             t.codes += done * K;
             t.scales += done * p.groups;
@@ -518,7 +534,6 @@ extern "C" int tc_gemm_tn_act8(const void *dy, long ld_dy, const void *codes, co
     } else {
         p.nk = (int)((M + KT - 1) / KT);
         p.tiles_k = (K + 127) / 128;
-        p.accumulate = w.slabs > 1 ? 0 : accumulate;
         TC_LAUNCH(gemm_tn8_kernel, small_grid, dim3(256), LDS_BYTES, s, p);
     }
     TC_CHECK_LAUNCH("tc_gemm_tn_act8");
