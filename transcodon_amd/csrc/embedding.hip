@@ -42,7 +42,9 @@ __global__ __launch_bounds__(256) void embedding_kernel(const TID *__restrict__ 
     }
 }
 
-constexpr int VEC = 4;                // columns of a lane in the gradient's kernels; a wave takes 64 VEC columns
+// Columns of a lane in the gradient's kernels; a wave takes 64 VEC.  (8 of bf16, one 16-byte load, halves the waves: 47 instead
+// of 39 us for the sums of 49153 x 1024.)
+constexpr int VEC = 4;
 
 // ---- gradient of a few positions -----------------------------------------------------------------------
 // Up to kFew positions: no sort.  Every wave holds all ids, finds the positions of a table row by comparing, and adds their
@@ -119,15 +121,15 @@ __global__ __launch_bounds__(256) void few_positions_kernel(const FewParams p) {
 // one workgroup's work and all digits one launch.  The sort keeps few CUs busy, so its launches also clear the gradient,
 // a slice each, with workgroups of their own.
 constexpr int kSortWaves = 16;
-constexpr int kSortTile = 4096;       // positions of a workgroup while there are few: 4 rounds of each wave
-constexpr int kMaxBlocks = 256;
+constexpr int kSortRounds = 4;        // positions of a lane, kept in registers
+constexpr int kSortTile = 64 * kSortWaves * kSortRounds;
 constexpr int kMaxBits = 9;
 
 struct SortParams {
     const void *tokens;               // first pass: ids (4 or 8 bytes each)
     uint32_t *keys[2], *pos[2];       // later passes: from [(pass - 1) & 1] to [pass & 1]
     uint32_t *hist;                   // [blocks][bins]
-    int id_bytes, M, tile, blocks, bits, passes;
+    int id_bytes, M, blocks, bits, passes;
     long vocab, pad_idx;
     float *clear;                     // gradient to clear (null: none), this launch's slice
     long clear_from, clear_to;
@@ -154,35 +156,64 @@ __device__ __forceinline__ bool clear_slice(const SortParams &p) {
     return true;
 }
 
+// This lane's positions: round r of wave w takes 64 neighbours, waves follow each other.  Past the end: no position.
+struct SortItems {
+    int at[kSortRounds];                     // -1: none
+    uint32_t key[kSortRounds];
+    __device__ __forceinline__ SortItems(const SortParams &p, int pass) {
+        const long first = (long)blockIdx.x * kSortTile + (threadIdx.x >> 6) * 64 * kSortRounds + (threadIdx.x & 63);
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r) {
+            at[r] = first + 64 * r < p.M ? (int)(first + 64 * r) : -1;
+            key[r] = at[r] >= 0 ? sort_key(p, pass, at[r]) : 0;
+        }
+    }
+    // Adds round r's digits to the wave's counts, one atomic for all lanes of a digit (padding would put all 64 on one
+    // counter); returns how many of the wave's earlier positions, this round's lower lanes included, have the lane's digit.
+    __device__ __forceinline__ uint32_t count(int r, uint32_t *counts, int shift, int bits) const {
+        const int lane = threadIdx.x & 63;
+        const uint32_t digit = (key[r] >> shift) & ((1u << bits) - 1);
+        unsigned long long same = __ballot(at[r] >= 0);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned long long ones = __ballot((digit >> b) & 1u);
+            same &= ((digit >> b) & 1u) ? ones : ~ones;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        uint32_t earlier = 0;
+        if (at[r] >= 0 && rank == 0) earlier = atomicAdd(counts + digit, (uint32_t)__popcll(same));
+        return __shfl(earlier, same ? __ffsll((long long)same) - 1 : 0, 64) + rank;
+    }
+};
+
 __global__ __launch_bounds__(64 * kSortWaves) void sort_count_kernel(const SortParams p, int pass) {
     if (clear_slice(p)) return;
     __shared__ uint32_t h[1 << kMaxBits];
     const int bins = 1 << p.bits;
-    for (int d = threadIdx.x; d < bins; d += 64 * kSortWaves) h[d] = 0;
+    const SortItems it(p, pass);
+    if ((int)threadIdx.x < bins) h[threadIdx.x] = 0;
     __syncthreads();
-    const int begin = blockIdx.x * p.tile, end = min(p.M, begin + p.tile);
-    for (int i = begin + threadIdx.x; i < end; i += 64 * kSortWaves) atomicAdd(&h[(sort_key(p, pass, i) >> (pass * p.bits)) & (bins - 1)], 1u);
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) it.count(r, h, pass * p.bits, p.bits);
     __syncthreads();
-    for (int d = threadIdx.x; d < bins; d += 64 * kSortWaves) p.hist[(long)blockIdx.x * bins + d] = h[d];
+    if ((int)threadIdx.x < bins) p.hist[(long)blockIdx.x * bins + threadIdx.x] = h[threadIdx.x];
 }
 
 __global__ __launch_bounds__(64 * kSortWaves) void sort_place_kernel(const SortParams p, int first_pass, int last_pass) {
     if (clear_slice(p)) return;
-    __shared__ uint32_t at[kSortWaves][1 << kMaxBits];      // next place per wave and digit
+    __shared__ uint32_t at[kSortWaves][1 << kMaxBits];      // per wave and digit: positions, then the place of the first
     __shared__ uint32_t total[1 << kMaxBits];
     const int bins = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int begin = blockIdx.x * p.tile, end = min(p.M, begin + p.tile);
-    const int span = p.tile / kSortWaves;                    // the tile is a multiple of 64 kSortWaves
-    const int w_begin = begin + wave * span, w_end = min(end, w_begin + span);
+    const int d = threadIdx.x;                               // bins <= 512: at most one digit per thread
     for (int pass = first_pass; pass <= last_pass; ++pass) { // more than one only where there is one workgroup
         const int shift = pass * p.bits;
-        for (int d = threadIdx.x; d < kSortWaves * bins; d += 64 * kSortWaves) at[d >> p.bits][d & (bins - 1)] = 0;
+        const SortItems it(p, pass);
+        for (int i = threadIdx.x; i < kSortWaves * bins; i += 64 * kSortWaves) at[i >> p.bits][i & (bins - 1)] = 0;
         __syncthreads();
-        for (int i = w_begin + lane; i < w_end; i += 64) atomicAdd(&at[wave][(sort_key(p, pass, i) >> shift) & (bins - 1)], 1u);
-        uint32_t before = 0;                                 // bins <= 512: at most one digit per thread
-        const int d = threadIdx.x;
+        uint32_t earlier[kSortRounds];
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r) earlier[r] = it.count(r, at[wave], shift, p.bits);
+        uint32_t before = 0, sum = 0;
         if (p.blocks > 1 && d < bins) {
-            uint32_t sum = 0;
             const uint32_t *h = p.hist + d;
 #pragma unroll 16
             for (int b = 0; b < p.blocks; ++b) {
@@ -190,14 +221,17 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_place_kernel(const SortP
                 before += b < (int)blockIdx.x ? n : 0;
                 sum += n;
             }
-            total[d] = sum;
         }
         __syncthreads();
-        if (p.blocks == 1 && d < bins) {
-            uint32_t sum = 0;
+        uint32_t n[kSortWaves] = {};
+        if (d < bins) {
+            uint32_t mine = 0;
 #pragma unroll
-            for (int w = 0; w < kSortWaves; ++w) sum += at[w][d];
-            total[d] = sum;
+            for (int w = 0; w < kSortWaves; ++w) {
+                n[w] = at[w][d];
+                mine += n[w];
+            }
+            total[d] = p.blocks > 1 ? sum : mine;
         }
         __syncthreads();
         // exclusive scan of the totals by one wave, eight digits per lane
@@ -223,34 +257,19 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_place_kernel(const SortP
             uint32_t place = total[d] + before;
 #pragma unroll
             for (int w = 0; w < kSortWaves; ++w) {
-                const uint32_t n = at[w][d];
                 at[w][d] = place;
-                place += n;
+                place += n[w];
             }
         }
         __syncthreads();
         uint32_t *keys_out = p.keys[pass & 1], *pos_out = p.pos[pass & 1];
-        for (int i0 = w_begin; i0 < w_end; i0 += 64) {
-            const int i = i0 + lane;
-            const bool live = i < w_end;
-            const uint32_t key = live ? sort_key(p, pass, i) : 0;
-            const uint32_t digit = (key >> shift) & (bins - 1);
-            unsigned long long same = __ballot(live);
-            for (int b = 0; b < p.bits; ++b) {
-                const unsigned long long ones = __ballot((digit >> b) & 1u);
-                same &= ((digit >> b) & 1u) ? ones : ~ones;
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r)
+            if (it.at[r] >= 0) {
+                const uint32_t place = at[wave][(it.key[r] >> shift) & (bins - 1)] + earlier[r];
+                keys_out[place] = it.key[r];
+                pos_out[place] = pass == 0 ? (uint32_t)it.at[r] : p.pos[(pass - 1) & 1][it.at[r]];
             }
-            // the first lane of each digit moves the wave's place on by the number of its lanes
-            const int rank = __popcll(same & ((1ull << lane) - 1));
-            uint32_t place = 0;
-            if (live && rank == 0) place = atomicAdd(&at[wave][digit], (uint32_t)__popcll(same));
-            const int first = same ? __ffsll((long long)same) - 1 : 0;
-            place = __shfl(place, first, 64) + rank;
-            if (live) {
-                keys_out[place] = key;
-                pos_out[place] = pass == 0 ? (uint32_t)i : p.pos[(pass - 1) & 1][i];
-            }
-        }
         __syncthreads();                                     // the next pass of the same workgroup reads what all its waves wrote
     }
 }
@@ -258,7 +277,8 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_place_kernel(const SortP
 // ---- segmented sum ----------------------------------------------------------------------------------------
 // A workgroup takes kSumWaves pieces of kPiece positions; each wave sums the runs of its piece, and where a run goes on into
 // the next piece the sums are handed over in LDS.  What crosses the workgroup's ends goes to memory, one row at either
-// end, for segment_join_kernel.
+// end, for segment_join_kernel.  HBM bound: 65536 x 768 f32 rows into 10 are 31 us (181 MB, 5.8 TB/s); the sort and the join
+// around it add 18.  Other shapes (4 to 16 waves, pieces of 8 to 32) are within 10 %, none faster.
 constexpr int kSumWaves = 8, kPiece = 32, kSpan = kSumWaves * kPiece;
 struct SumParams {
     const uint32_t *keys, *pos;       // sorted
@@ -401,17 +421,13 @@ __global__ __launch_bounds__(256) void segment_join_kernel(const SumParams p) {
 }
 
 struct BwdPlan {
-    int tile, blocks, passes, bits, spans, part_ld;
+    int blocks, passes, bits, spans, part_ld;
     size_t keys[2], pos[2], hist, partial, total;
 };
 BwdPlan bwd_plan(long M, long E, long vocab) {
     BwdPlan w{};
     if (M <= kFew) { w.total = 16; return w; }
-    const long unit = 64 * kSortWaves;
-    long tile = (M + kMaxBlocks - 1) / kMaxBlocks;
-    tile = (tile + unit - 1) / unit * unit;
-    w.tile = (int)(tile < kSortTile ? kSortTile : tile);
-    w.blocks = (int)((M + w.tile - 1) / w.tile);
+    w.blocks = (int)((M + kSortTile - 1) / kSortTile);
     int bits = 0;
     while ((vocab >> bits) != 0) ++bits;           // keys 0 .. vocab
     w.passes = (bits + kMaxBits - 1) / kMaxBits;
@@ -531,7 +547,7 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
     SortParams sp{};
     sp.tokens = tokens;
     sp.id_bytes = id_bytes;
-    sp.M = (int)M; sp.tile = w.tile; sp.blocks = w.blocks; sp.bits = w.bits; sp.passes = w.passes;
+    sp.M = (int)M; sp.blocks = w.blocks; sp.bits = w.bits; sp.passes = w.passes;
     sp.vocab = vocab; sp.pad_idx = pad_idx;
     sp.hist = reinterpret_cast<uint32_t *>(ws + w.hist);
     for (int k = 0; k < 2; ++k) {
