@@ -244,7 +244,7 @@ __global__ __launch_bounds__(256) void attn_bwd_dq_bf16_kernel(const BwdParams p
             }
         }
 
-        // P = exp2(S log2e - lse log2e), dS = P (dP - delta): packed f32 arithmetic; padded keys get
+        // P = exp2(S log2e - lse log2e), dS = P (dP - delta), two values at a time; padded keys get
         // S = -inf first (only in tiles that contain one: wave-uniform branch)
         const uint64_t word = s_words[kt];
         if (word != ~0ull) {

@@ -106,7 +106,7 @@ __device__ __forceinline__ float gelu_fast(float x) {
     return 0.5f * x * (x < 0.f ? erfc_abs : 2.0f - erfc_abs);
 }
 
-// Two values at a time: the polynomial and the scalings map onto packed f32 VALU ops.
+// Two values at a time: two independent chains of the polynomial.
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 __device__ __forceinline__ f32x2 gelu_fast2(f32x2 x) {
     const f32x2 ax = {fabsf(x[0]), fabsf(x[1])};
