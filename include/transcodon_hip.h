@@ -475,6 +475,8 @@ typedef struct tc_encoder_desc {
     int32_t num_layers, E, F, H, vocab, n_species, n_struct, pad_idx;
     int32_t rope_table_len;       /* rows in every rope_cos/rope_sin table (>= T)      */
     float ln_eps;
+    int32_t act8;                 /* training, bf16 only: 1 = the inputs of q/k/v, fc1 and gelu are kept for the backward
+                                   * pass in 8 bits (see tc_act8_pack); 0 = in bf16                                    */
     const float *tok_table;       /* embed_tokens.weight [vocab,E] f32                 */
     const float *species_table;   /* species_embedding.weight [n_species,E] f32        */
     const tc_layer_weights *layers; /* host array [num_layers]                          */
@@ -608,7 +610,13 @@ typedef struct tc_encoder_grads {
     float *st_bias;         /* gradient of both structure_linear.out_proj.bias and .bias */
 } tc_encoder_grads;
 
-/* Bytes of workspace for tc_encoder_forward_train + tc_encoder_backward on a [B,T] batch. */
+/*
+ * Bytes of workspace for tc_encoder_forward_train + tc_encoder_backward on a [B,T] batch.  With desc->act8 the two LayerNorm
+ * outputs and the fc1 pre-activation of each layer are kept as e4m3 codes with one power of two per 32 values and gelu's output
+ * not at all: 22 E + 4 H bytes a token and layer instead of 36 E + 4 H (F = 4 E).  The forward pass computes the same values either way; the
+ * gradients see the rounded ones (weight gradients of q/k/v, fc1 and fc2, and gelu').  desc->act8 must be the same in
+ * all three calls.
+ */
 size_t tc_train_workspace_bytes(const tc_encoder_desc *desc, int B, int T);
 
 /*

@@ -31,7 +31,7 @@ class EncoderDesc(C.Structure):
     _fields_ = (
         [(n, C.c_int32) for n in ("dtype", "num_layers", "E", "F", "H", "vocab", "n_species",
                                   "n_struct", "pad_idx", "rope_table_len")]
-        + [("ln_eps", C.c_float)]
+        + [("ln_eps", C.c_float), ("act8", C.c_int32)]
         + [(n, vp) for n in ("tok_table", "species_table")]
         + [("layers", C.POINTER(LayerWeights))]
         + [(n, vp) for n in ("lnf_g", "lnf_b", "w_heads", "b_heads", "lm_ln_g", "lm_ln_b",

@@ -18,6 +18,8 @@ struct LayerSaved {
     void *h2;        // LayerNorm 2 output                            dtype [M,E]
     void *u;         // fc1 pre-activation                            dtype [M,F]
     void *mid;       // gelu(u)                                       dtype [M,F]
+    // instead of h1, h2, u and mid with desc->act8: 8-bit form of h1, h2 and u
+    void *h1_c, *h1_s, *h2_c, *h2_s, *u_c, *u_s;
 };
 
 constexpr int kMaxLayers = 64;
@@ -82,14 +84,20 @@ TrainWs carve(const tc_encoder_desc *d, int B, int T, char *base) {
     for (int l = 0; l < d->num_layers && l < kMaxLayers; ++l) {
         LayerSaved &s = w.L[l];
         s.x_in = reinterpret_cast<float *>(take(M * E * 4));
-        s.h1 = take(M * E * esz);
+        if (d->act8) {
+            s.h1_c = take(M * E); s.h1_s = take(M * ((E + 31) / 32));
+            s.h2_c = take(M * E); s.h2_s = take(M * ((E + 31) / 32));
+            s.u_c = take(M * F); s.u_s = take(M * ((F + 31) / 32));
+        } else {
+            s.h1 = take(M * E * esz);
+            s.h2 = take(M * E * esz);
+            s.u = take(M * ldf * esz);
+            s.mid = take(M * ldf * esz);
+        }
         s.qkv = take(M * 3 * E * esz);
         s.ao = take(M * E * esz);
         s.lse = reinterpret_cast<float *>(take((size_t)B * d->H * T * 4));
         s.x_mid = reinterpret_cast<float *>(take(M * E * 4));
-        s.h2 = take(M * E * esz);
-        s.u = take(M * ldf * esz);
-        s.mid = take(M * ldf * esz);
     }
     w.x = reinterpret_cast<float *>(take(M * E * 4));
     w.hf = take(M * E * esz);
@@ -112,6 +120,12 @@ TrainWs carve(const tc_encoder_desc *d, int B, int T, char *base) {
         const size_t v = (size_t)wgrad_splits(d->dtype, (int)sh[0], (int)sh[1], nk) * sh[0] * sh[1];
         if (v > sf) sf = v;
     }
+    if (d->act8) {
+        for (const size_t n_out : {3 * E, F}) {
+            const size_t v = tc_gemm_tn_act8_workspace_bytes((long)M, (long)n_out, (int)n_out, (int)E) / 4;
+            if (v > sf) sf = v;
+        }
+    }
     w.slab_floats = sf;
     w.slabs = reinterpret_cast<float *>(take(sf * 4));
     w.delta = reinterpret_cast<float *>(take((size_t)B * d->H * T * 4));
@@ -122,6 +136,7 @@ TrainWs carve(const tc_encoder_desc *d, int B, int T, char *base) {
 int check_desc(const tc_encoder_desc *d, const char *who) {
     TC_REQUIRE(d != nullptr, "%s: null descriptor", who);
     TC_REQUIRE(d->dtype == TC_BF16 || d->dtype == TC_F32, "%s: bad dtype %d", who, d->dtype);
+    TC_REQUIRE(!d->act8 || d->dtype == TC_BF16, "%s: 8-bit activations are for bf16", who);
     TC_REQUIRE(d->num_layers > 0 && d->num_layers <= kMaxLayers && d->layers, "%s: bad layer count", who);
     TC_REQUIRE(d->E > 0 && d->H > 0 && d->E == d->H * 64, "%s: E=%d H=%d needs head_dim 64", who, d->E, d->H);
     TC_REQUIRE(d->E % 128 == 0 && d->F % 128 == 0 && d->E <= 768, "%s: E=%d (<= 768) and F=%d must be multiples of 128",
@@ -172,6 +187,13 @@ int linear_wgrad(const tc_encoder_desc *d, TrainWs &w, int in_dt, const void *dy
     return TC_OK;
 }
 
+// The same with X kept in 8 bits (bf16 dY): codes and scales straight into the product.
+int linear_wgrad8(TrainWs &w, const void *dy, int ld_dy, const void *codes, const void *scales, int M, int n_out, int n_in, float *dW,
+                  float *dbias, void *stream) {
+    TC_TRY(tc_colsum(TC_BF16, dy, ld_dy, nullptr, 0, dbias, M, n_out, stream));
+    return tc_gemm_tn_act8(dy, ld_dy, codes, scales, dW, M, n_out, n_in, 1, w.slabs, w.slab_floats * sizeof(float), stream);
+}
+
 // Transposed weights, wt[n_in, n_out] = W[n_out, n_in]^T: the "weight" operand of the data-gradient products dX = dY W.
 // Layer l keeps q/k/v, out-proj, fc1, fc2 in this order; the two head dense matrices follow the last layer.
 enum { WT_QKV = 0, WT_O = 1, WT_FC1 = 2, WT_FC2 = 3 };
@@ -211,7 +233,7 @@ int transpose_weights(const tc_encoder_desc *d, const TrainWs &w, void *stream) 
 }  // namespace
 
 extern "C" size_t tc_train_workspace_bytes(const tc_encoder_desc *desc, int B, int T) {
-    if (!desc || B <= 0 || T <= 0 || desc->num_layers > kMaxLayers) return 0;
+    if (!desc || B <= 0 || T <= 0 || desc->num_layers > kMaxLayers || (desc->act8 && desc->dtype != TC_BF16)) return 0;
     return carve(desc, B, T, nullptr).total;
 }
 
@@ -249,16 +271,22 @@ extern "C" int tc_encoder_forward_train(const tc_encoder_desc *d, const int32_t 
         TC_REQUIRE(lw.ln1_g && lw.ln1_b && lw.w_qkv && lw.b_qkv && lw.w_o && lw.b_o && lw.ln2_g && lw.ln2_b &&
                        lw.w_fc1 && lw.b_fc1 && lw.w_fc2 && lw.b_fc2 && lw.rope_cos && lw.rope_sin,
                    "tc_encoder_forward_train: layer %d has a null weight pointer", l);
-        TC_TRY(ln(sv.x_in, lw.ln1_g, lw.ln1_b, sv.h1));
-        TC_TRY(tc_gemm(dt, TC_EPI_QKV_ROPE, sv.h1, E, lw.w_qkv, lw.b_qkv, nullptr, sv.qkv, 3 * E, M, 3 * E, E, 0.125f,
+        // with 8-bit activations the bf16 ones live in the backward pass's temporaries until the next product has read them
+        void *h1 = d->act8 ? w.dyb : sv.h1, *h2 = d->act8 ? w.dyb : sv.h2;
+        void *u = d->act8 ? w.wide : sv.u, *mid = d->act8 ? w.tr_a : sv.mid;
+        TC_TRY(ln(sv.x_in, lw.ln1_g, lw.ln1_b, h1));
+        if (d->act8) TC_TRY(tc_act8_pack(dt, h1, E, sv.h1_c, sv.h1_s, M, E, stream));
+        TC_TRY(tc_gemm(dt, TC_EPI_QKV_ROPE, h1, E, lw.w_qkv, lw.b_qkv, nullptr, sv.qkv, 3 * E, M, 3 * E, E, 0.125f,
                        lw.rope_cos, lw.rope_sin, T, 64, stream));
         TC_TRY(tc_attn_fwd_train(dt, sv.qkv, 3 * E, w.words, sv.ao, sv.lse, B, T, d->H, 64, stream));
         TC_TRY(tc_gemm(dt, TC_EPI_BIAS_RESIDUAL, sv.ao, E, lw.w_o, lw.b_o, sv.x_in, sv.x_mid, E, M, E, E, 0.f, nullptr,
                        nullptr, 0, 0, stream));
-        TC_TRY(ln(sv.x_mid, lw.ln2_g, lw.ln2_b, sv.h2));
-        TC_TRY(tc_gemm_train(dt, TC_EPI_BIAS_GELU_SAVE, sv.h2, E, lw.w_fc1, lw.b_fc1, nullptr, sv.mid, sv.u, w.ld_f, M, F,
-                             E, 1, stream));
-        TC_TRY(tc_gemm(dt, TC_EPI_BIAS_RESIDUAL, sv.mid, w.ld_f, lw.w_fc2, lw.b_fc2, sv.x_mid, x_next, E, M, E, F, 0.f,
+        TC_TRY(ln(sv.x_mid, lw.ln2_g, lw.ln2_b, h2));
+        if (d->act8) TC_TRY(tc_act8_pack(dt, h2, E, sv.h2_c, sv.h2_s, M, E, stream));
+        TC_TRY(tc_gemm_train(dt, TC_EPI_BIAS_GELU_SAVE, h2, E, lw.w_fc1, lw.b_fc1, nullptr, mid, u, w.ld_f, M, F, E, 1,
+                             stream));
+        if (d->act8) TC_TRY(tc_act8_pack(dt, u, w.ld_f, sv.u_c, sv.u_s, M, F, stream));
+        TC_TRY(tc_gemm(dt, TC_EPI_BIAS_RESIDUAL, mid, w.ld_f, lw.w_fc2, lw.b_fc2, sv.x_mid, x_next, E, M, E, F, 0.f,
                        nullptr, nullptr, 0, 0, stream));
     }
     TC_TRY(ln(w.x, d->lnf_g, d->lnf_b, w.hf));
@@ -362,18 +390,31 @@ extern "C" int tc_encoder_backward_notify(const tc_encoder_desc *d, const tc_enc
         const tc_layer_grads &lg = g->layers[l];
         LayerSaved &sv = w.L[l];
         // ---- feed-forward block: x_out = x_mid + fc2(gelu(fc1(LN2(x_mid)))) ----
-        if (fuse)
-            TC_TRY(linear_wgrad(d, w, TC_BF16, w.dyb, E, nullptr, sv.mid, w.ld_f, M, E, F, lg.w_fc2, nullptr, stream));
-        else
-            TC_TRY(linear_wgrad(d, w, TC_F32, dx, E, w.dyb, sv.mid, w.ld_f, M, E, F, lg.w_fc2, lg.b_fc2, stream));
-        // fc1's bias gradient is summed in the epilogue that produces d_u (bf16 mode)
-        TC_TRY(tc_gemm_train(dt, TC_EPI_DGELU, w.dyb, E, wt_of(d, w, l, WT_FC2), nullptr, sv.u, w.wide, fuse ? lg.b_fc1 : nullptr, w.ld_f, M,
-                             F, E, 1, stream));
-        TC_TRY(linear_wgrad(d, w, dt, w.wide, w.ld_f, nullptr, sv.h2, E, M, F, E, lg.w_fc1, fuse ? nullptr : lg.b_fc1,
-                            stream));
+        const void *du = w.wide;       // gradient of fc1's output
+        int ld_du = w.ld_f;
+        if (d->act8) {
+            // gelu's output again and its gradient, from the 8-bit input in one pass; both are dense in the transposes' buffers
+            TC_TRY(tc_gemm(dt, TC_EPI_BIAS, w.dyb, E, wt_of(d, w, l, WT_FC2), nullptr, nullptr, w.wide, w.ld_f, M, F, E, 0.f, nullptr,
+                           nullptr, 0, 0, stream));
+            TC_TRY(tc_dgelu_act8(dt, w.wide, w.ld_f, sv.u_c, sv.u_s, w.tr_a, w.tr_b, M, F, stream));
+            du = w.tr_a;
+            ld_du = F;
+            TC_TRY(linear_wgrad(d, w, TC_BF16, w.dyb, E, nullptr, w.tr_b, F, M, E, F, lg.w_fc2, nullptr, stream));
+            TC_TRY(linear_wgrad8(w, du, ld_du, sv.h2_c, sv.h2_s, M, F, E, lg.w_fc1, lg.b_fc1, stream));
+        } else {
+            if (fuse)
+                TC_TRY(linear_wgrad(d, w, TC_BF16, w.dyb, E, nullptr, sv.mid, w.ld_f, M, E, F, lg.w_fc2, nullptr, stream));
+            else
+                TC_TRY(linear_wgrad(d, w, TC_F32, dx, E, w.dyb, sv.mid, w.ld_f, M, E, F, lg.w_fc2, lg.b_fc2, stream));
+            // fc1's bias gradient is summed in the epilogue that produces d_u (bf16 mode)
+            TC_TRY(tc_gemm_train(dt, TC_EPI_DGELU, w.dyb, E, wt_of(d, w, l, WT_FC2), nullptr, sv.u, w.wide, fuse ? lg.b_fc1 : nullptr, w.ld_f, M,
+                                 F, E, 1, stream));
+            TC_TRY(linear_wgrad(d, w, dt, w.wide, w.ld_f, nullptr, sv.h2, E, M, F, E, lg.w_fc1, fuse ? nullptr : lg.b_fc1,
+                                stream));
+        }
         // the gradient handed to a LayerNorm comes out of the product in the compute type (bf16: what a
         // bf16 Linear returns under autocast), half the bytes for the product to write and the LayerNorm to read
-        TC_TRY(tc_gemm(dt, TC_EPI_BIAS, w.wide, w.ld_f, wt_of(d, w, l, WT_FC1), nullptr, nullptr, w.t0, E, M, E, F, 0.f, nullptr, nullptr, 0,
+        TC_TRY(tc_gemm(dt, TC_EPI_BIAS, du, ld_du, wt_of(d, w, l, WT_FC1), nullptr, nullptr, w.t0, E, M, E, F, 0.f, nullptr, nullptr, 0,
                        0, stream));
         TC_TRY(tc_layernorm_bwd_dy(TC_F32, sv.x_mid, E, lw.ln2_g, dt, w.t0, E, dx, 1, lg.ln2_g, lg.ln2_b,
                                    fuse ? w.dyb : nullptr, fuse ? lg.b_o : nullptr, M, E, d->ln_eps, stream));
@@ -387,7 +428,10 @@ extern "C" int tc_encoder_backward_notify(const tc_encoder_desc *d, const tc_enc
                        stream));
         TC_TRY(tc_attn_bwd(dt, sv.qkv, 3 * E, w.words, sv.ao, d_ao, sv.lse, w.delta, w.wide, 3 * E, lw.rope_cos,
                            lw.rope_sin, 0.125f, B, T, d->H, 64, stream));
-        TC_TRY(linear_wgrad(d, w, dt, w.wide, 3 * E, nullptr, sv.h1, E, M, 3 * E, E, lg.w_qkv, lg.b_qkv, stream));
+        if (d->act8)
+            TC_TRY(linear_wgrad8(w, w.wide, 3 * E, sv.h1_c, sv.h1_s, M, 3 * E, E, lg.w_qkv, lg.b_qkv, stream));
+        else
+            TC_TRY(linear_wgrad(d, w, dt, w.wide, 3 * E, nullptr, sv.h1, E, M, 3 * E, E, lg.w_qkv, lg.b_qkv, stream));
         TC_TRY(tc_gemm(dt, TC_EPI_BIAS, w.wide, 3 * E, wt_of(d, w, l, WT_QKV), nullptr, nullptr, w.t0, E, M, E, 3 * E, 0.f, nullptr, nullptr,
                        0, 0, stream));
         const bool below = fuse && l > 0;    // layer 0 hands dx to the embedding backward only

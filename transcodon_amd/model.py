@@ -76,6 +76,7 @@ class ProteinBertModel(nn.Module):
         self.compute_dtype = None       # None: follow the parameter dtype (f32 unless .bfloat16())
         self.check_indices = True       # raise IndexError on out-of-range token / species ids
         self.fold_layernorm = True      # bf16 inference: LayerNorms of the layers folded into the products
+        self.act8_checkpoints = False   # training in bf16: activations kept for the backward pass in 8 bits
         self._pack = {}
         self._workspace = None
         self._train_workspace = None

@@ -131,6 +131,10 @@ class EncoderTrainFunction(torch.autograd.Function):
         dt = model._dtype()
         pk = model._packed(dt, T, dev)
         lib = _lib.load()
+        act8 = int(bool(model.act8_checkpoints))
+        if act8 and dt != torch.bfloat16:
+            raise ValueError("act8_checkpoints needs the bf16 compute type (set_compute_dtype(torch.bfloat16))")
+        pk["desc"].act8 = act8
         need = lib.tc_train_workspace_bytes(C.byref(pk["desc"]), B, T)
         if need == 0:
             raise _lib.HipLibraryError("tc_train_workspace_bytes: unsupported configuration")
@@ -146,6 +150,7 @@ class EncoderTrainFunction(torch.autograd.Function):
         model._train_generation += 1
         ctx.model, ctx.pk, ctx.ws, ctx.tok32, ctx.sp32 = model, pk, ws, tok32, sp32
         ctx.generation = model._train_generation
+        ctx.act8 = act8
         ctx.set_materialize_grads(False)
         return logits, struct
 
@@ -170,6 +175,7 @@ class EncoderTrainFunction(torch.autograd.Function):
             gp = _GradPack(model, dev)
             struct = gp.struct
         sync = getattr(store, "grad_sync", None) if gp is None else None
+        ctx.pk["desc"].act8 = ctx.act8       # as the forward saved them, whatever the model's switch says by now
         args = (C.byref(ctx.pk["desc"]), C.byref(struct), ctx.tok32.data_ptr(), ctx.sp32.data_ptr(), B, T,
                 dlogits.data_ptr(), None if dstruct is None else dstruct.data_ptr(), ctx.ws.data_ptr(),
                 ctx.ws.numel())
