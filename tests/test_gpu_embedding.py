@@ -120,6 +120,22 @@ def test_gradient_adds_to_a_given_buffer_and_takes_strided_rows():
 
 
 @gpu
+@pytest.mark.parametrize("rows", [50, 333, 6000])
+def test_gradient_into_a_buffer_that_is_aligned_to_a_value_only(rows):
+    gen = torch.Generator().manual_seed(rows)
+    vocab, width = 40, 64
+    tok, dy = torch.randint(0, vocab, (rows,), generator=gen).to(DEV), torch.randn(rows, width, generator=gen).to(DEV)
+    want = ops.embedding_bwd(tok, dy, vocab)
+    store = torch.full((vocab * width + 9,), 5.0, device=DEV)
+    out = store[3:3 + vocab * width].view(vocab, width)
+    out.zero_()
+    assert torch.equal(ops.embedding_bwd(tok, dy, vocab, out=out), want)
+    assert bool((store[:3] == 5).all()) and bool((store[3 + vocab * width:] == 5).all())
+    table = store[3:3 + vocab * width].view(vocab, width)
+    assert torch.equal(ops.embedding(tok, table), table[tok])
+
+
+@gpu
 def test_gradient_is_that_of_differences():
     """The lookup is linear in its table: moving one entry by d moves <dy, out> by d * gradient."""
     gen = torch.Generator().manual_seed(7)
@@ -163,6 +179,10 @@ def test_refusals():
         ops.embedding_bwd(tok, dy.t().contiguous().t(), 3)
     with pytest.raises(ValueError):
         ops.embedding_bwd(tok, dy, 3, out=torch.zeros(4, 8, device=DEV))
+    for call in (lambda: ops.embedding(tok, table, pad_idx=-1), lambda: ops.embedding_bwd(tok, dy, 3, pad_idx=-1),
+                 lambda: ops.embedding_bwd(tok, dy[:1].expand(4, 8), 3)):
+        with pytest.raises(ValueError):
+            call()
     with pytest.raises(_lib.HipLibraryError):
         ops.embedding_bwd(tok, dy, 0)
 

@@ -198,6 +198,24 @@ def test_backward_without_one_of_the_gradients(pre, dxo):
 
 
 @gpu
+@pytest.mark.parametrize("M,E", [(37, 768), (37, 771), (9000, 96)])
+def test_backward_of_strided_rows(M, E):
+    c = _case(M, E, torch.bfloat16, 1, False)
+    x_out = _forward(c, False, 1.0)[0].float()
+    g = _on_gpu(c)
+    stats = _stats64(c, x_out, False).to(DEV)
+    rest = (stats, g["post_gamma"], g["post_beta"], g["gate"], g["pre_gamma"], g["pre_beta"])
+    want = ops.gated_residual_norm_bwd(g["dh"], g["dx_out"], g["y"], x_out.to(DEV), *rest)
+    for first in (4, 3):                                          # 3: rows no aligned vector load fits
+        def wide(t):
+            w = torch.full((M, E + 12), float("nan"), dtype=t.dtype, device=DEV)
+            w[:, first:first + E] = t.to(DEV)
+            return w[:, first:first + E]
+        got = ops.gated_residual_norm_bwd(wide(g["dh"]), wide(g["dx_out"]), wide(g["y"]), wide(x_out), *rest)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
 @pytest.mark.parametrize("G", [1, 5, 300])
 def test_backward_adds_to_given_buffers(G):
     c = _case(300, 132, torch.float32, G, False)

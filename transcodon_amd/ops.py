@@ -366,6 +366,13 @@ def _rows(t, name):
     raise ValueError(f"{name} must be 2-d with unit column stride and rows that do not overlap")
 
 
+def _scratch(need, out, dev):
+    """Workspace of ``need`` bytes; 16 stand for "none is used", where the output's address does."""
+    if need <= 16 and out.data_ptr() % 16 == 0:
+        return out
+    return torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+
+
 def _dense(t, name, shape=None, dtype=None):
     """Checks a dense operand: its shape and element type where they are given."""
     if not t.is_contiguous():
@@ -374,6 +381,14 @@ def _dense(t, name, shape=None, dtype=None):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} has type {t.dtype}, expected {dtype}")
+
+
+def _pad(pad_idx):
+    if pad_idx is None:
+        return -1
+    if pad_idx < 0:
+        raise ValueError(f"pad_idx must be None or at least 0, got {pad_idx}")
+    return pad_idx
 
 
 def _id_bytes(tokens):
@@ -402,7 +417,7 @@ def embedding(tokens, table, scale=1.0, pad_idx=None, out_dtype=None, bad=None):
     dts = _dt(table), _dt(out)
     if M and E:
         _call("tc_embedding_fwd", dev, *dts, idb, tokens.data_ptr(), table.data_ptr(), out.data_ptr(), M, E, V, scale,
-              -1 if pad_idx is None else pad_idx, _p(bad))
+              _pad(pad_idx), _p(bad))
     return out
 
 
@@ -426,9 +441,9 @@ def embedding_bwd(tokens, dy, vocab, scale=1.0, pad_idx=None, out=None):
     dt = _dt(dy)
     if M and E:
         need = _lib.load().tc_embedding_bwd_workspace_bytes(M, E, vocab)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        ws = _scratch(need, out, dev)
         _call("tc_embedding_bwd", dev, dt, idb, tokens.data_ptr(), dy.data_ptr(), ld, out.data_ptr(), M, E, vocab, scale,
-              -1 if pad_idx is None else pad_idx, int(accumulate), ws.data_ptr(), need)
+              _pad(pad_idx), int(accumulate), ws.data_ptr(), need)
     return out
 
 
@@ -624,7 +639,7 @@ def gemm_tn_act8(dy, codes, scales, out=None):
         out = torch.empty(N, K, dtype=torch.float32, device=dev)
     if M:
         need = _lib.load().tc_gemm_tn_act8_workspace_bytes(M, ld, N, K)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        ws = _scratch(need, out, dev)
         _call("tc_gemm_tn_act8", dev, dy.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), M, N, K,
               int(accumulate), ws.data_ptr(), need)
     return out
