@@ -724,7 +724,7 @@ int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, const void 
  * norm(t) = (t - mean(t)) / sqrt(var(t) + eps), or with rms != 0 t / sqrt(mean(t^2) + eps).
  * y, h: dtype (f32 or bf16); x, x_out and the vectors: f32; gate: f32, or bf16 with bf16 rows, [G,E] where row g is
  * for rows g M/G .. (g+1) M/G - 1 (G = 1: one for all, G = M: one for each; gate NULL and G = 0: none).  The betas may be NULL;
- * pre_gamma, pre_beta and h NULL leave the second norm out.  y and x may have row strides ldy, ldx >= E; x_out may be x.
+ * pre_gamma, pre_beta and h NULL leave the second norm out.  y and x may have row strides ldy, ldx >= E; x_out may be x where ldx is E.
  * stats (optional) [M,4] f32: mean and 1/deviation of y, then of x_out (0, 0 without the second norm).  E <= 8192.
  */
 int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, const float *x, long ldx, const float *post_gamma,
@@ -734,7 +734,7 @@ int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, const float *
 
 /*
  * Its gradient.  dh (dtype; NULL without the second norm) and dx_out (f32; may be NULL) are the gradients of h and
- * x_out, y, x_out and stats those of the forward pass.  Writes dy (dtype) and dx (f32; may be dx_out) dense, and the f32
+ * x_out, y, x_out and stats those of the forward pass.  Writes dy (dtype) and dx (f32; may be dx_out where ld_dxo is E) dense, and the f32
  * gradients of the vectors and of the gate [G,E] (d_gate goes with gate; the others may be NULL).  accumulate: bits 0 .. 4 add to
  * d_post_gamma, d_post_beta, d_pre_gamma, d_pre_beta, d_gate instead of overwriting them.  Column sums have a fixed order:
  * the result is the same every time.
@@ -758,7 +758,7 @@ int tc_act8_pack(int dtype, const void *x, long ldx, void *codes, void *scales, 
 int tc_act8_unpack(int dtype, const void *codes, const void *scales, void *out, long M, int E, void *stream);
 /* act = gelu(u) (exact erf form, transcodon/modules.py:17-24) and the 8-bit form of u in one pass */
 int tc_gelu_act8(int dtype, const void *u, long ldu, void *act, void *codes, void *scales, long M, int E, void *stream);
-/* du = dy * gelu'(v) and, unless act is NULL, act = gelu(v), v being what the codes stand for.  du may be dy (dense). */
+/* du = dy * gelu'(v) and, unless act is NULL, act = gelu(v), v being what the codes stand for.  du may be dy where ld_dy is E. */
 int tc_dgelu_act8(int dtype, const void *dy, long ld_dy, const void *codes, const void *scales, void *du, void *act, long M, int E,
                   void *stream);
 /*

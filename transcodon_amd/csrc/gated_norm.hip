@@ -13,6 +13,7 @@
 // neighbouring rows and keeps the column sums (gradients of the norms' vectors and of the gate) in registers; teams of
 // a workgroup are added in LDS, workgroups by a second kernel, always in the same order.
 #include "row_io.h"
+#include <math.h>
 
 namespace {
 
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(1024) void gated_norm_join_kernel(const NormParams 
         if (!out) continue;
         float s = 0.f;
         if (col < p.E)
-#pragma unroll 4
+#pragma unroll 8
             for (int i = r; i < n; i += 16) s += src[i * ld + col];
         red[r][c] = s;
         __syncthreads();
@@ -408,15 +409,15 @@ __global__ __launch_bounds__(1024) void gated_norm_join_kernel(const NormParams 
 
 // How a row is laid over lanes: W waves a row, NC loads of VEC values a lane and operand.  Rows whose width or addresses do
 // not allow aligned loads take the LOOSE form: unaligned ones, and the values of a row's end one by one.
-// One wave a row needs no barrier and is the faster form for many rows (65536 x 768 bf16: forward 115 against 150 us with
-// four waves, backward 208 against 228; 8192 rows: forward 16.5 / 19.6, backward 33.0 / 32.4).  With few rows, or rows of narrow loads,
-// it leaves the chip idle: 4101 x 770 f32 backward 47 us with one wave, 29 with four.
-constexpr long kManyRows = 8192;
+// One wave a row needs no barrier; four waves bring more of the chip to few rows.  Where they meet, bf16 rows of 768:
+// forward 131 rows 4.4 / 3.9 us (one / four waves), 1024 rows 5.0 / 5.4, 65536 rows 115 / 150; backward 8192 rows
+// 39 / 31, 16384 rows 56 / 47, 32768 rows 113 / 121, 65536 rows 208 / 228.
+constexpr long kManyRowsFwd = 512, kManyRowsBwd = 24576;
 struct Shape {
     int W, nc;
 };
-Shape row_shape(long M, int E) {
-    const int W = E <= 1024 && M >= kManyRows ? 1 : E <= 2048 ? 4 : E <= 4096 ? 8 : 16;
+Shape row_shape(long M, int E, long many) {
+    const int W = E <= 1024 && M >= many ? 1 : E <= 2048 ? 4 : E <= 4096 ? 8 : 16;
     return Shape{W, (E + 64 * VEC * W - 1) / (64 * VEC * W)};
 }
 
@@ -427,10 +428,16 @@ struct BwdPlan {
 BwdPlan bwd_plan(int M, int E, int G, int W) {
     BwdPlan w{};
     const int per_wg = W == 1 ? 4 : 1;
-    // Teams: enough to fill the chip once.  One wave a row: 2048 waves are 210 us at 65536 x 768 bf16 (1024: 245, 3072: 252, 4096: 215).
-    // Four waves: 1024 workgroups are 28.7 us at 4101 x 770 f32 (512: 29.5, 2048: 32.8: every workgroup leaves 4 E sums).
+    // Teams: at most as many as fill the chip once.  One wave a row: 2048 waves are 210 us at 65536 x 768 bf16 (1024: 245, 3072: 252,
+    // 4096: 215).  Several waves: every workgroup leaves 4 E sums to be written and joined, 12 us for 1024 of them, and every
+    // further row costs a workgroup 1 us, so rows * 1 us + M / rows * 12 ns is least at the root of M / 85 (1024 x 768 bf16: 1
+    // row 18.9 us, 2 13.7, 4 12.7, 8 15.9).
     const int want = W == 1 ? 2048 : 4096 / W;
-    const int rows = (int)(((long)M + want - 1) / want);
+    int rows = (int)(((long)M + want - 1) / want);
+    if (W > 1) {
+        const int even = (int)(sqrt((double)M / 85.0) + 0.5);
+        rows = rows > even ? rows : even;
+    }
     const int group = G > 0 ? M / G : 0;
     if (G == 0 || group <= rows) {
         w.rows_per_team = G == 0 ? rows : rows / group * group;
@@ -509,7 +516,7 @@ extern "C" int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, co
     const bool loose = !(tc_rows_aligned(y, ldy, esz, VEC) && tc_rows_aligned(x, ldx, 4, VEC) && tc_rows_aligned(gate, E, g_esz, VEC) &&
                tc_rows_aligned(h, E, esz, VEC) && tc_rows_aligned(x_out, E, 4, VEC) && tc_rows_aligned(post_gamma, 0, 4, VEC) &&
                tc_rows_aligned(post_beta, 0, 4, VEC) && tc_rows_aligned(pre_gamma, 0, 4, VEC) && tc_rows_aligned(pre_beta, 0, 4, VEC));
-    const Shape sh = row_shape(M, E);
+    const Shape sh = row_shape(M, E, kManyRowsFwd);
     const int per_wg = sh.W == 1 ? 4 : 1;
     long blocks = (M + per_wg - 1) / per_wg;
     // rows are walked with the grid's stride: a launch holds fewer than 2^32 threads, and teams that ask ahead fill the chip once
@@ -567,7 +574,7 @@ extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh,
                (!dh || tc_rows_aligned(dh, ld_dh, esz, VEC)) && (!dx_out || tc_rows_aligned(dx_out, ld_dxo, 4, VEC)) &&
                tc_rows_aligned(dy, E, esz, VEC) && tc_rows_aligned(dx, E, 4, VEC) && tc_rows_aligned(d_gate, E, 4, VEC) &&
                tc_rows_aligned(post_gamma, 0, 4, VEC) && tc_rows_aligned(post_beta, 0, 4, VEC) && tc_rows_aligned(pre_gamma, 0, 4, VEC));
-    const Shape sh = row_shape(M, E);
+    const Shape sh = row_shape(M, E, kManyRowsBwd);
     const BwdPlan w = bwd_plan((int)M, E, G, sh.W);
     NormParams p{};
     p.y = y; p.x = x_out; p.gate = gate; p.dh = dh; p.dx_out = dx_out;
