@@ -9,7 +9,7 @@
 //
 // A team of W waves owns a row at a time and keeps it in registers, so every operand is read from memory once; deviations are
 // summed after the mean is known.  HBM bound: 65536 x 768 in bf16 with 64 gate rows 115 us forward (604 MB, 5.3 TB/s; a
-// large copy: 4.9) and 208 us backward (907 MB, 4.35 TB/s).  The backward pass gives each team a run of
+// large copy: 4.9) and 194 us backward (907 MB, 4.7 TB/s).  The backward pass gives each team a run of
 // neighbouring rows and keeps the column sums (gradients of the norms' vectors and of the gate) in registers; teams of
 // a workgroup are added in LDS, workgroups by a second kernel, always in the same order.
 #include "row_io.h"
@@ -216,10 +216,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
     }
     if (t >= p.teams) begin = end = 0;
     const float inv_e = 1.0f / (float)p.E;
-    // A row's operands as they were loaded.  The next row is requested before this one is worked on: three dependent row
-    // reductions per row leave a wave idle otherwise, and the registers allow only two or three waves a SIMD.  (Not with
-    // 16 waves, which leave 128 registers each, or 16 values a lane: there the second row would not fit.)
-    constexpr bool kAhead = NC * VEC <= 12 && W < 16;
+    // A row's operands as they were loaded.  The next row is requested before this one is worked on, since three dependent
+    // row reductions leave a wave idle otherwise, and the vectors stay in registers, the gate's row until its group ends
+    // (loading them again for every row: 65536 x 768 bf16 208 instead of 194 us).  Sixteen waves leave 128 registers each,
+    // which hold neither.
+    constexpr bool kAhead = W < 16, kKeep = W < 16;
     struct Row {
         typename TcRaw<T, VEC>::type y[NC], dh[NC];
         typename TcRaw<float, VEC>::type x[NC], d[NC];
@@ -244,6 +245,18 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
         next.y[c] = next.dh[c] = typename TcRaw<T, VEC>::type{};
         next.x[c] = next.d[c] = typename TcRaw<float, VEC>::type{};
     }
+    float kg1[NC][VEC], kb1[NC][VEC], kg2[NC][VEC], kgt[NC][VEC];
+    long kept_gate = -1;
+    if (kKeep) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = col0 + c * 64 * W * VEC;
+            if (n[c] == 0) continue;
+            tc_load_row<float, VEC, LOOSE>(p.g1 + col, kg1[c], n[c]);
+            if (p.gate && p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + col, kb1[c], n[c]);
+            if (p.g2) tc_load_row<float, VEC, LOOSE>(p.g2 + col, kg2[c], n[c]);
+        }
+    }
     if (kAhead && begin < end) request(begin);
     for (long row = begin; row < end; ++row) {
         if (!kAhead) request(row);
@@ -264,9 +277,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
                 const int col = col0 + c * 64 * W * VEC;
                 if (n[c] == 0) continue;
                 float g[VEC];
-                tc_load_row<float, VEC, LOOSE>(p.g2 + col, g, n[c]);
+                if (!kKeep) tc_load_row<float, VEC, LOOSE>(p.g2 + col, g, n[c]);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
+                    if (kKeep) g[j] = kg2[c][j];
                     const float xh = (xv[c][j] - st[2]) * st[3];
                     acc[2][c][j] += dh[c][j] * xh;
                     acc[3][c][j] += dh[c][j];
@@ -285,17 +299,27 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
                 for (int j = 0; j < VEC; ++j) d[c][j] += st[3] * (dh[c][j] - m1 - xv[c][j] * m2);
         }
         const long gate_row = (long)((unsigned)row / (unsigned)p.rows_per_gate) * p.E;      // rows are below 2^31
+        if (kKeep && p.gate && gate_row != kept_gate) {
+            kept_gate = gate_row;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (n[c] > 0)
+                    tc_load_row<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + gate_row + col0 + c * 64 * W * VEC, kgt[c], n[c]);
+        }
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int col = col0 + c * 64 * W * VEC;
             if (n[c] == 0) continue;
             float g[VEC], b[VEC], gt[VEC], o[VEC];
-            tc_load_row<float, VEC, LOOSE>(p.g1 + col, g, n[c]);
-            if (p.gate) tc_load_row<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + gate_row + col, gt, n[c]);
-            if (p.gate && p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + col, b, n[c]);
+            if (!kKeep) {
+                tc_load_row<float, VEC, LOOSE>(p.g1 + col, g, n[c]);
+                if (p.gate) tc_load_row<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + gate_row + col, gt, n[c]);
+                if (p.gate && p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + col, b, n[c]);
+            }
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
+                if (kKeep) { g[j] = kg1[c][j]; b[j] = kb1[c][j]; gt[j] = kgt[c][j]; }
                 const float yh = (yv[c][j] - st[0]) * st[1];
                 float dn = d[c][j];
                 if (p.gate) {
@@ -409,29 +433,32 @@ __global__ __launch_bounds__(1024) void gated_norm_join_kernel(const NormParams 
 
 // How a row is laid over lanes: W waves a row, NC loads of VEC values a lane and operand.  Rows whose width or addresses do
 // not allow aligned loads take the LOOSE form: unaligned ones, and the values of a row's end one by one.
-// One wave a row needs no barrier; four waves bring more of the chip to few rows.  Where they meet, bf16 rows of 768:
-// forward 131 rows 4.4 / 3.9 us (one / four waves), 1024 rows 5.0 / 5.4, 65536 rows 115 / 150; backward 8192 rows
-// 39 / 31, 16384 rows 56 / 47, 32768 rows 113 / 121, 65536 rows 208 / 228.
-constexpr long kManyRowsFwd = 512, kManyRowsBwd = 24576;
+// One wave a row needs no barrier; four waves bring more of the chip to few rows and leave registers for rows ahead.
+// Forward, bf16 rows of 768, one / four waves: 131 rows 4.4 / 3.9 us, 1024 rows 5.0 / 5.4, 65536 rows 115 / 150.
+// Backward, 16384 rows: 256 wide 25 / 32, 384 33 / 34, 512 38 / 35, 768 49 / 44, 1024 83 / 67; 65536 rows: 256 wide 79 / 117, 512 135 / 150,
+// 640 171 / 171, 768 197 / 195, 1024 273 / 261.
 struct Shape {
     int W, nc;
 };
-Shape row_shape(long M, int E, long many) {
-    const int W = E <= 1024 && M >= many ? 1 : E <= 2048 ? 4 : E <= 4096 ? 8 : 16;
+Shape row_shape(int E, bool one_wave) {
+    const int W = one_wave ? 1 : E <= 2048 ? 4 : E <= 4096 ? 8 : 16;
     return Shape{W, (E + 64 * VEC * W - 1) / (64 * VEC * W)};
 }
+Shape fwd_shape(long M, int E) { return row_shape(E, E <= 1024 && M >= 512); }
+Shape bwd_shape(int E) { return row_shape(E, E <= 512); }
 
 struct BwdPlan {
     int teams, rows_per_team, teams_per_group, workgroups;
     size_t bytes;
 };
-BwdPlan bwd_plan(int M, int E, int G, int W) {
+BwdPlan bwd_plan(int M, int E, int G) {
     BwdPlan w{};
+    const int W = bwd_shape(E).W;
     const int per_wg = W == 1 ? 4 : 1;
-    // Teams: at most as many as fill the chip once.  One wave a row: 2048 waves are 210 us at 65536 x 768 bf16 (1024: 245, 3072: 252,
-    // 4096: 215).  Several waves: every workgroup leaves 4 E sums to be written and joined, 12 us for 1024 of them, and every
-    // further row costs a workgroup 1 us, so rows * 1 us + M / rows * 12 ns is least at the root of M / 85 (1024 x 768 bf16: 1
-    // row 18.9 us, 2 13.7, 4 12.7, 8 15.9).
+    // Teams: at most as many as fill the chip once (65536 x 768 bf16, four waves: 1024 teams 195 us, 768 219, 1536 237, 2048 202).
+    // Several waves: every workgroup leaves 4 E sums to be written and joined, 12 us for 1024 of them, and every further row
+    // costs a workgroup 1 us, so rows * 1 us + M / rows * 12 ns is least at the root of M / 85 (1024 x 768 bf16: 1 row 18.9 us,
+    // 2 13.7, 4 12.7, 8 15.9).
     const int want = W == 1 ? 2048 : 4096 / W;
     int rows = (int)(((long)M + want - 1) / want);
     if (W > 1) {
@@ -464,23 +491,30 @@ int check_common(const char *who, int dtype, int gate_dtype, const void *gate, l
 
 }  // namespace
 
-#define TC_GN_W(K, T, TG, LOOSE)                                                                \
-    do {                                                                                        \
-        switch (sh.W * 10 + sh.nc) {                                                            \
+// the shapes that fwd_shape and bwd_shape name, as W * 10 + NC
+#define TC_GN_COMMON(K, T, TG, LOOSE)                                                           \
             case 11: TC_GN(K, T, TG, LOOSE, 1, 1); break;                                       \
             case 12: TC_GN(K, T, TG, LOOSE, 1, 2); break;                                       \
-            case 13: TC_GN(K, T, TG, LOOSE, 1, 3); break;                                       \
-            case 14: TC_GN(K, T, TG, LOOSE, 1, 4); break;                                       \
             case 41: TC_GN(K, T, TG, LOOSE, 4, 1); break;                                       \
             case 42: TC_GN(K, T, TG, LOOSE, 4, 2); break;                                       \
             case 82: TC_GN(K, T, TG, LOOSE, 8, 2); break;                                       \
-            default: TC_GN(K, T, TG, LOOSE, 16, 2); break;                                      \
+            default: TC_GN(K, T, TG, LOOSE, 16, 2); break;
+#define TC_GN_FWD(T, TG, LOOSE)                                                                 \
+    do {                                                                                        \
+        switch (sh.W * 10 + sh.nc) {                                                            \
+            case 13: TC_GN(gated_norm_kernel, T, TG, LOOSE, 1, 3); break;                       \
+            case 14: TC_GN(gated_norm_kernel, T, TG, LOOSE, 1, 4); break;                       \
+            TC_GN_COMMON(gated_norm_kernel, T, TG, LOOSE)                                       \
         }                                                                                       \
+    } while (0)
+#define TC_GN_BWD(T, TG, LOOSE)                                                                 \
+    do {                                                                                        \
+        switch (sh.W * 10 + sh.nc) { TC_GN_COMMON(gated_norm_bwd_kernel, T, TG, LOOSE) }        \
     } while (0)
 #define TC_GN_L(K, T, TG)                                                                       \
     do {                                                                                        \
-        if (loose) TC_GN_W(K, T, TG, true);                                                     \
-        else TC_GN_W(K, T, TG, false);                                                          \
+        if (loose) K(T, TG, true);                                                              \
+        else K(T, TG, false);                                                                   \
     } while (0)
 #define TC_GN_T(K)                                                                              \
     do {                                                                                        \
@@ -516,7 +550,7 @@ extern "C" int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, co
     const bool loose = !(tc_rows_aligned(y, ldy, esz, VEC) && tc_rows_aligned(x, ldx, 4, VEC) && tc_rows_aligned(gate, E, g_esz, VEC) &&
                tc_rows_aligned(h, E, esz, VEC) && tc_rows_aligned(x_out, E, 4, VEC) && tc_rows_aligned(post_gamma, 0, 4, VEC) &&
                tc_rows_aligned(post_beta, 0, 4, VEC) && tc_rows_aligned(pre_gamma, 0, 4, VEC) && tc_rows_aligned(pre_beta, 0, 4, VEC));
-    const Shape sh = row_shape(M, E, kManyRowsFwd);
+    const Shape sh = fwd_shape(M, E);
     const int per_wg = sh.W == 1 ? 4 : 1;
     long blocks = (M + per_wg - 1) / per_wg;
     // rows are walked with the grid's stride: a launch holds fewer than 2^32 threads, and teams that ask ahead fill the chip once
@@ -525,7 +559,7 @@ extern "C" int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, co
     hipStream_t s = static_cast<hipStream_t>(stream);
     TcProfScope prof(TC_PROF_LAYERNORM, s, (double)M * E * (2 * esz + 8));
 #define TC_GN(K, T, TG, L, WW, N) TC_LAUNCH((K<T, TG, L, WW, N>), dim3((unsigned)blocks), dim3(WW == 1 ? 256 : 64 * WW), 0, s, p)
-    TC_GN_T(gated_norm_kernel);
+    TC_GN_T(TC_GN_FWD);
 #undef TC_GN
     TC_CHECK_LAUNCH("tc_gated_residual_norm_fwd");
     return TC_OK;
@@ -533,13 +567,7 @@ extern "C" int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, co
 
 extern "C" size_t tc_gated_residual_norm_bwd_workspace_bytes(long M, int E, int G) {
     if (M <= 0 || M > 0x7fffffffL || E <= 0 || E > 8192 || G < 0 || (G > 0 && M % G != 0)) return 0;
-    // which layout a call takes depends on its addresses too: enough for each
-    size_t most = 16;
-    for (int W : {1, 4, 8, 16}) {
-        const size_t n = bwd_plan((int)M, E, G, W).bytes;
-        most = n > most ? n : most;
-    }
-    return most;
+    return bwd_plan((int)M, E, G).bytes;
 }
 
 extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh, const float *dx_out, long ld_dxo, const void *y,
@@ -574,8 +602,8 @@ extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh,
                (!dh || tc_rows_aligned(dh, ld_dh, esz, VEC)) && (!dx_out || tc_rows_aligned(dx_out, ld_dxo, 4, VEC)) &&
                tc_rows_aligned(dy, E, esz, VEC) && tc_rows_aligned(dx, E, 4, VEC) && tc_rows_aligned(d_gate, E, 4, VEC) &&
                tc_rows_aligned(post_gamma, 0, 4, VEC) && tc_rows_aligned(post_beta, 0, 4, VEC) && tc_rows_aligned(pre_gamma, 0, 4, VEC));
-    const Shape sh = row_shape(M, E, kManyRowsBwd);
-    const BwdPlan w = bwd_plan((int)M, E, G, sh.W);
+    const Shape sh = bwd_shape(E);
+    const BwdPlan w = bwd_plan((int)M, E, G);
     NormParams p{};
     p.y = y; p.x = x_out; p.gate = gate; p.dh = dh; p.dx_out = dx_out;
     p.stats = const_cast<float *>(stats);
@@ -593,7 +621,7 @@ extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh,
     TcProfScope prof(TC_PROF_LAYERNORM, s, (double)M * E * (3 * esz + 12));
 #define TC_GN(K, T, TG, L, WW, N)                                                                                         \
     TC_LAUNCH((K<T, TG, L, WW, N>), dim3((unsigned)w.workgroups), dim3(WW == 1 ? 256 : 64 * WW), WW == 1 ? 16 * (size_t)E : 0, s, p)
-    TC_GN_T(gated_norm_bwd_kernel);
+    TC_GN_T(TC_GN_BWD);
 #undef TC_GN
     const int groups = w.teams_per_group > 0 ? G : 0;
     const int tall = 4 + groups < 1024 ? 4 + groups : 1024;
