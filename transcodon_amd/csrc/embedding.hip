@@ -121,14 +121,15 @@ __global__ __launch_bounds__(256) void few_positions_kernel(const FewParams p) {
 // one workgroup's work and all digits one launch.  The sort keeps few CUs busy, so its launches also clear the gradient,
 // a slice each, with workgroups of their own.
 constexpr int kSortWaves = 16;
-constexpr int kSortRounds = 4;        // positions of a lane, kept in registers
-constexpr int kSortTile = 64 * kSortWaves * kSortRounds;
+constexpr int kSortThreads = 64 * kSortWaves;
 constexpr int kMaxBits = 9;
+constexpr int kFewBlocks = 128;
 
 struct SortParams {
     const void *tokens;               // first pass: ids (4 or 8 bytes each)
     uint32_t *keys[2], *pos[2];       // later passes: from [(pass - 1) & 1] to [pass & 1]
     uint32_t *hist;                   // [blocks][bins]
+    uint32_t *totals;                 // [bins], with hist already summed over the workgroups before (null: not yet)
     int id_bytes, M, blocks, bits, passes;
     long vocab, pad_idx;
     float *clear;                     // gradient to clear (null: none), this launch's slice
@@ -144,9 +145,9 @@ __device__ __forceinline__ uint32_t sort_key(const SortParams &p, int pass, int 
 // true for the workgroups behind the sorting ones, after they have cleared their part
 __device__ __forceinline__ bool clear_slice(const SortParams &p) {
     if ((int)blockIdx.x < p.blocks) return false;
-    const long n = p.clear_to - p.clear_from, step = (long)(gridDim.x - p.blocks) * 64 * kSortWaves;
+    const long n = p.clear_to - p.clear_from, step = (long)(gridDim.x - p.blocks) * kSortThreads;
     float *out = p.clear + p.clear_from;
-    const long first = (long)(blockIdx.x - p.blocks) * 64 * kSortWaves + threadIdx.x;
+    const long first = (long)(blockIdx.x - p.blocks) * kSortThreads + threadIdx.x;
     if (((uintptr_t)out & 15) == 0) {
         for (long i = first; i < n / 4; i += step) *reinterpret_cast<f32x4 *>(out + 4 * i) = f32x4{0.f, 0.f, 0.f, 0.f};
         for (long i = n / 4 * 4 + first; i < n; i += step) out[i] = 0.f;
@@ -157,13 +158,14 @@ __device__ __forceinline__ bool clear_slice(const SortParams &p) {
 }
 
 // This lane's positions: round r of wave w takes 64 neighbours, waves follow each other.  Past the end: no position.
+template <int R>                             // rounds: positions of a lane, kept in registers
 struct SortItems {
-    int at[kSortRounds];                     // -1: none
-    uint32_t key[kSortRounds];
+    int at[R];                               // -1: none
+    uint32_t key[R];
     __device__ __forceinline__ SortItems(const SortParams &p, int pass) {
-        const long first = (long)blockIdx.x * kSortTile + (threadIdx.x >> 6) * 64 * kSortRounds + (threadIdx.x & 63);
+        const long first = (long)blockIdx.x * kSortThreads * R + (threadIdx.x >> 6) * 64 * R + (threadIdx.x & 63);
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) {
+        for (int r = 0; r < R; ++r) {
             at[r] = first + 64 * r < p.M ? (int)(first + 64 * r) : -1;
             key[r] = at[r] >= 0 ? sort_key(p, pass, at[r]) : 0;
         }
@@ -185,20 +187,51 @@ struct SortItems {
     }
 };
 
-__global__ __launch_bounds__(64 * kSortWaves) void sort_count_kernel(const SortParams p, int pass) {
+template <int R>
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortParams p, int pass) {
     if (clear_slice(p)) return;
     __shared__ uint32_t h[1 << kMaxBits];
     const int bins = 1 << p.bits;
-    const SortItems it(p, pass);
+    const SortItems<R> it(p, pass);
     if ((int)threadIdx.x < bins) h[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) it.count(r, h, pass * p.bits, p.bits);
+    for (int r = 0; r < R; ++r) it.count(r, h, pass * p.bits, p.bits);
     __syncthreads();
     if ((int)threadIdx.x < bins) p.hist[(long)blockIdx.x * bins + threadIdx.x] = h[threadIdx.x];
 }
 
-__global__ __launch_bounds__(64 * kSortWaves) void sort_place_kernel(const SortParams p, int first_pass, int last_pass) {
+// Counts of many workgroups: each becomes the sum over the workgroups before, the whole sum goes to totals.  64 digits a
+// workgroup, 16 row lanes that take a run of the counts each.
+__global__ __launch_bounds__(kSortThreads) void sort_scan_kernel(const SortParams p) {
+    __shared__ uint32_t part[kSortWaves][64];
+    const int bins = 1 << p.bits, c = threadIdx.x & 63, r = threadIdx.x >> 6;
+    const int d = blockIdx.x * 64 + c;
+    const int len = (p.blocks + kSortWaves - 1) / kSortWaves, begin = min(p.blocks, r * len), end = min(p.blocks, begin + len);
+    uint32_t sum = 0;
+    if (d < bins)
+#pragma unroll 8
+        for (int b = begin; b < end; ++b) sum += p.hist[(long)b * bins + d];
+    part[r][c] = sum;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (int w = 0; w < kSortWaves; ++w) {
+        before += w < r ? part[w][c] : 0;
+        all += part[w][c];
+    }
+    if (d < bins) {
+        if (r == 0) p.totals[d] = all;
+#pragma unroll 8
+        for (int b = begin; b < end; ++b) {
+            const uint32_t n = p.hist[(long)b * bins + d];
+            p.hist[(long)b * bins + d] = before;
+            before += n;
+        }
+    }
+}
+
+template <int R>
+__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortParams p, int first_pass, int last_pass) {
     if (clear_slice(p)) return;
     __shared__ uint32_t at[kSortWaves][1 << kMaxBits];      // per wave and digit: positions, then the place of the first
     __shared__ uint32_t total[1 << kMaxBits];
@@ -206,14 +239,17 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_place_kernel(const SortP
     const int d = threadIdx.x;                               // bins <= 512: at most one digit per thread
     for (int pass = first_pass; pass <= last_pass; ++pass) { // more than one only where there is one workgroup
         const int shift = pass * p.bits;
-        const SortItems it(p, pass);
-        for (int i = threadIdx.x; i < kSortWaves * bins; i += 64 * kSortWaves) at[i >> p.bits][i & (bins - 1)] = 0;
+        const SortItems<R> it(p, pass);
+        for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) at[i >> p.bits][i & (bins - 1)] = 0;
         __syncthreads();
-        uint32_t earlier[kSortRounds];
+        uint32_t earlier[R];
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) earlier[r] = it.count(r, at[wave], shift, p.bits);
+        for (int r = 0; r < R; ++r) earlier[r] = it.count(r, at[wave], shift, p.bits);
         uint32_t before = 0, sum = 0;
-        if (p.blocks > 1 && d < bins) {
+        if (p.totals && d < bins) {
+            before = p.hist[(long)blockIdx.x * bins + d];
+            sum = p.totals[d];
+        } else if (p.blocks > 1 && d < bins) {
             const uint32_t *h = p.hist + d;
 #pragma unroll 16
             for (int b = 0; b < p.blocks; ++b) {
@@ -264,7 +300,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_place_kernel(const SortP
         __syncthreads();
         uint32_t *keys_out = p.keys[pass & 1], *pos_out = p.pos[pass & 1];
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r)
+        for (int r = 0; r < R; ++r)
             if (it.at[r] >= 0) {
                 const uint32_t place = at[wave][(it.key[r] >> shift) & (bins - 1)] + earlier[r];
                 keys_out[place] = it.key[r];
@@ -278,7 +314,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_place_kernel(const SortP
 // A workgroup takes kSumWaves pieces of kPiece positions; each wave sums the runs of its piece, and where a run goes on into
 // the next piece the sums are handed over in LDS.  What crosses the workgroup's ends goes to memory, one row at either
 // end, for segment_join_kernel.  HBM bound: 65536 x 768 f32 rows into 10 are 31 us (181 MB, 5.8 TB/s); the sort and the join
-// around it add 18.  Other shapes (4 to 16 waves, pieces of 8 to 32) are within 10 %, none faster.
+// around it add 14.  Other shapes (4 to 16 waves, pieces of 8 to 32) are within 10 %, none faster.
 constexpr int kSumWaves = 8, kPiece = 32, kSpan = kSumWaves * kPiece;
 struct SumParams {
     const uint32_t *keys, *pos;       // sorted
@@ -421,13 +457,17 @@ __global__ __launch_bounds__(256) void segment_join_kernel(const SumParams p) {
 }
 
 struct BwdPlan {
-    int blocks, passes, bits, spans, part_ld;
-    size_t keys[2], pos[2], hist, partial, total;
+    int rounds, blocks, passes, bits, spans, part_ld;
+    size_t keys[2], pos[2], hist, totals, partial, total;
 };
 BwdPlan bwd_plan(long M, long E, long vocab) {
     BwdPlan w{};
     if (M <= kFew) { w.total = 16; return w; }
-    w.blocks = (int)((M + kSortTile - 1) / kSortTile);
+    // A workgroup scatters its positions line by line, so few of them are dealt to many workgroups: up to 131072 rows 1 round each
+    // (65536 rows of 64 into 50000: 38 us, with 4 rounds 49).  Up to kFewBlocks workgroups each sums the counts of the others by
+    // itself, which is one launch less; with more of them that grows with the square.
+    w.rounds = M <= 4 * kSortThreads || M > kFewBlocks * kSortThreads ? 4 : 1;
+    w.blocks = (int)((M + kSortThreads * w.rounds - 1) / (kSortThreads * w.rounds));
     int bits = 0;
     while ((vocab >> bits) != 0) ++bits;           // keys 0 .. vocab
     w.passes = (bits + kMaxBits - 1) / kMaxBits;
@@ -442,6 +482,7 @@ BwdPlan bwd_plan(long M, long E, long vocab) {
     };
     for (int k = 0; k < 2; ++k) { w.keys[k] = take((size_t)M * 4); w.pos[k] = take((size_t)M * 4); }
     w.hist = take((size_t)w.blocks * (1 << w.bits) * 4);
+    w.totals = take((size_t)(1 << w.bits) * 4);
     w.partial = take((size_t)w.spans * 2 * w.part_ld * 4);
     w.total = off;
     return w;
@@ -550,6 +591,7 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
     sp.M = (int)M; sp.blocks = w.blocks; sp.bits = w.bits; sp.passes = w.passes;
     sp.vocab = vocab; sp.pad_idx = pad_idx;
     sp.hist = reinterpret_cast<uint32_t *>(ws + w.hist);
+    if (w.blocks > kFewBlocks) sp.totals = reinterpret_cast<uint32_t *>(ws + w.totals);
     for (int k = 0; k < 2; ++k) {
         sp.keys[k] = reinterpret_cast<uint32_t *>(ws + w.keys[k]);
         sp.pos[k] = reinterpret_cast<uint32_t *>(ws + w.pos[k]);
@@ -566,16 +608,22 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
         const long wgs = (sp.clear_to - sp.clear_from + 16383) / 16384;
         return dim3((unsigned)(w.blocks + (wgs < 512 ? wgs : 512)));
     };
-    for (int pass = 0; pass < w.passes; ++pass) {
-        dim3 grid = grid_of();
-        if (w.blocks == 1) {
-            TC_LAUNCH(sort_place_kernel, grid, dim3(64 * kSortWaves), 0, s, sp, 0, w.passes - 1);
-            break;
+#define TC_SORT(KERNEL, ...)                                                                                    \
+    do {                                                                                                        \
+        const dim3 grid = grid_of();                                                                            \
+        if (w.rounds == 1) TC_LAUNCH(KERNEL<1>, grid, dim3(kSortThreads), 0, s, sp, __VA_ARGS__);               \
+        else TC_LAUNCH(KERNEL<4>, grid, dim3(kSortThreads), 0, s, sp, __VA_ARGS__);                             \
+    } while (0)
+    if (w.blocks == 1) {
+        TC_SORT(sort_place_kernel, 0, w.passes - 1);
+    } else {
+        for (int pass = 0; pass < w.passes; ++pass) {
+            TC_SORT(sort_count_kernel, pass);
+            if (sp.totals) TC_LAUNCH(sort_scan_kernel, dim3((unsigned)(((1 << w.bits) + 63) / 64)), dim3(kSortThreads), 0, s, sp);
+            TC_SORT(sort_place_kernel, pass, pass);
         }
-        TC_LAUNCH(sort_count_kernel, grid, dim3(64 * kSortWaves), 0, s, sp, pass);
-        grid = grid_of();
-        TC_LAUNCH(sort_place_kernel, grid, dim3(64 * kSortWaves), 0, s, sp, pass, pass);
     }
+#undef TC_SORT
     SumParams q{};
     q.keys = sp.keys[(w.passes - 1) & 1]; q.pos = sp.pos[(w.passes - 1) & 1];
     q.dy = dy; q.ld_dy = ld_dy;
