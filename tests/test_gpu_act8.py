@@ -288,3 +288,22 @@ def test_refusals_without_a_gpu():
     for bad in (dict(dy=None), dict(ld=4), dict(ld=12), dict(dy=one + 2), dict(codes=one + 8), dict(N=12), dict(K=24), dict(M=0), dict(ws=None)):
         assert tn(**bad) == -1, bad
     assert tn(n=need - 1) == -3
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 128 * 64])
+def test_weight_gradient_takes_scales_of_any_byte(rows):
+    """One row of ones among rows of zeros, every scale byte in it: 0 stands for 2^-127, 255 for NaN."""
+    N, K = 2048, 256 * 32
+    codes = torch.full((rows, K), 1.5, device=DEV).to(torch.float8_e4m3fn)
+    scales = torch.full((rows, 256), 127, dtype=torch.uint8, device=DEV)
+    scales[rows // 2] = torch.arange(256, dtype=torch.uint8, device=DEV)
+    scales = scales.view(torch.float8_e8m0fnu)
+    dy = torch.zeros(rows, N, dtype=torch.bfloat16, device=DEV)
+    dy[rows // 2] = 1.0
+    got = ops.gemm_tn_act8(dy, codes, scales)
+    want = ops.act8_unpack(codes[rows // 2:rows // 2 + 1], scales[rows // 2:rows // 2 + 1], torch.float32).expand(N, K)
+    assert bool(torch.isnan(got[:, 255 * 32:]).all())
+    # a product with a value below the smallest normal number may count as zero on the matrix cores
+    assert bool(((got[:, :255 * 32] - want[:, :255 * 32]).abs() <= 2.0 ** -126).all())
+    assert torch.equal(got[:, 2 * 32:255 * 32], want[:, 2 * 32:255 * 32])
