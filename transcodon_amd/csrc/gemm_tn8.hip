@@ -422,6 +422,25 @@ __global__ __launch_bounds__(512) void gemm_tn8_256_kernel(const Tn8Params p) {
         }
 }
 
+// Sum of many parts of a small gradient: 64 columns of four values a workgroup, 16 waves that take every 16th part each and
+// are added in order.  (tc_reduce_slabs gives a thread all parts of its values, one load after the other.)
+__global__ __launch_bounds__(1024) void tn8_sum_kernel(const float *__restrict__ slabs, float *__restrict__ out, int S, long n4, int accumulate) {
+    __shared__ f32x4 red[16][64];
+    const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
+    const long i = (long)blockIdx.x * 64 + c;
+    f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (i < n4)
+#pragma unroll 8
+        for (int k = r; k < S; k += 16) sum += *reinterpret_cast<const f32x4 *>(slabs + 4 * (k * n4 + i));
+    red[r][c] = sum;
+    __syncthreads();
+    if (r == 0 && i < n4) {
+        for (int k = 1; k < 16; ++k) sum += red[k][c];
+        if (accumulate) sum += *reinterpret_cast<const f32x4 *>(out + 4 * i);
+        *reinterpret_cast<f32x4 *>(out + 4 * i) = sum;
+    }
+}
+
 bool tn8_dims_ok(long M, int N, int K) {
     return M > 0 && M <= 0x7fffffffL - KT && N > 0 && K > 0 && N % 8 == 0 && K % 16 == 0 && N <= (1 << 20) && K <= (1 << 20) &&
            (long)((N + 127) / 128) * ((K + 127) / 128) <= (1 << 22);
@@ -431,18 +450,18 @@ struct Tn8Plan {
     bool big;                // 256 x 256 tiles over the whole stages, the rows behind them by the small kernel
     int splits, slabs;
 };
-// Which kernel and how many row splits: the least estimated time over both kernels and 1 .. 64 splits, in nanoseconds.
+constexpr int kManySlabs = 16;
+// Which kernel and how many row splits: the least estimated time over both kernels and up to 256 splits, in nanoseconds.
 // A stage takes a large tile 1.9 us on a full chip (220 us at 65536 x 2304 x 768: 114 stages), a small one 1 us while
 // there is one workgroup per CU and 0.6 us more for each further one; a part of the sum costs its slab written and read at
-// 6.5 TB/s, and more than one the summing launch.  Measured on either side of the rule: 262 x 768 x 768 in one part 10.0 us, in
-// five 14.7; 1024 x 768 x 768 in three 16.2, in sixteen 26.6; 65536 x 256 x 512 in 64 parts 55 us, in four 276.
+// 6.5 TB/s, and more than one the summing launch.
 Tn8Plan tn8_plan(long M, long ld_dy, int N, int K) {
     Tn8Plan best{};
     long least = -1;
     const long nk = (M + KT - 1) / KT, whole = M / KT;
     const long large = (long)((N + 255) / 256) * ((K + 255) / 256), small = (long)((N + 127) / 128) * ((K + 127) / 128);
     auto parts = [&](long slabs) { return slabs > 1 ? 4000 + slabs * N * K * 8 / 6500 : 0; };
-    for (long s = 1; s <= 64; ++s) {
+    for (long s = 1; s <= 256; s += s < 16 ? 1 : s < 64 ? 4 : 16) {
         if (s <= nk) {
             const long wgs = small * s;
             const long ns = 2000 + (nk + s - 1) / s * (400 + 600 * (wgs > 256 ? wgs : 256) / 256) + parts(s);
@@ -536,6 +555,10 @@ extern "C" int tc_gemm_tn_act8(const void *dy, long ld_dy, const void *codes, co
         p.tiles_k = (K + 127) / 128;
         TC_LAUNCH(gemm_tn8_kernel, small_grid, dim3(256), LDS_BYTES, s, p);
     }
+    if (w.slabs > kManySlabs) {
+        const long n4 = (long)N * K / 4;
+        TC_LAUNCH(tn8_sum_kernel, dim3((unsigned)((n4 + 63) / 64)), dim3(1024), 0, s, p.out, dW, w.slabs, n4, accumulate);
+    }
     TC_CHECK_LAUNCH("tc_gemm_tn_act8");
-    return w.slabs > 1 ? tc_reduce_slabs(p.out, dW, w.slabs, (long)N * K, accumulate, stream) : TC_OK;
+    return w.slabs > 1 && w.slabs <= kManySlabs ? tc_reduce_slabs(p.out, dW, w.slabs, (long)N * K, accumulate, stream) : TC_OK;
 }
