@@ -68,7 +68,8 @@ def test_lookup_flags_ids_out_of_range():
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab,width", [
     (1, 1, 1), (1, 1438, 768), (2, 2, 4), (63, 10, 768), (64, 10, 768), (65, 10, 768), (128, 3, 256), (129, 1, 260), (1023, 1438, 770),
-    (1024, 255, 96), (1025, 256, 33), (4096, 511, 64), (5000, 512, 64), (256, 50, 260), (257, 50, 260), (4097, 40, 8), (8191, 1000, 512), (9001, 70000, 40), (20000, 10, 768), (140000, 600, 8), (600000, 5000, 4), (2500000, 3, 1), (300000, 300000, 4)])
+    (1024, 255, 96), (1025, 256, 33), (4096, 511, 64), (5000, 512, 64), (256, 50, 260), (257, 50, 260), (511, 9, 65), (512, 300, 128), (513, 300, 128), (700, 524286, 4), (700, 524287, 4), (700, 524288, 4),
+    (4097, 40, 8), (8191, 1000, 512), (8192, 70000, 12), (8193, 70000, 12), (9001, 70000, 40), (20000, 10, 768), (140000, 600, 8), (600000, 5000, 4), (2500000, 3, 1), (300000, 300000, 4)])
 @pytest.mark.parametrize("kind", ["even", "one", "few"])
 def test_gradient(dt, rows, vocab, width, kind):
     gen = torch.Generator().manual_seed(rows + 3 * width)

@@ -49,7 +49,7 @@ constexpr int VEC = 4;
 // ---- gradient of a few positions -----------------------------------------------------------------------
 // Up to kFew positions: no sort.  Every wave holds all ids, finds the positions of a table row by comparing, and adds their
 // rows of dy in order; rows without a position are written as zeros on the way.
-constexpr int kFew = 256;
+constexpr int kFew = 512;
 struct FewParams {
     const void *tokens, *dy;
     float *out;
@@ -78,8 +78,9 @@ __global__ __launch_bounds__(256) void few_positions_kernel(const FewParams p) {
         for (int k = 0; k < kFew / 64; ++k) {
             unsigned long long left = __ballot(id[k] == v);
             any |= left != 0;
-            while (left) {
-                constexpr int U = 8;                               // rows in flight; a spent mask repeats its last row
+            // U rows in flight; a spent mask repeats its last row
+            auto batch = [&](auto u_c) {
+                constexpr int U = decltype(u_c)::value;
                 int at[U], n = 0;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
@@ -100,6 +101,10 @@ __global__ __launch_bounds__(256) void few_positions_kernel(const FewParams p) {
                     if (u < n)
 #pragma unroll
                         for (int j = 0; j < VEC; ++j) acc[j] += x[u][j];
+            };
+            while (left) {
+                if (__popcll(left) > 4) batch(std::integral_constant<int, 16>{});
+                else batch(std::integral_constant<int, 4>{});
             }
         }
         if (!in || (p.accumulate && !any)) continue;
@@ -117,8 +122,8 @@ __global__ __launch_bounds__(256) void few_positions_kernel(const FewParams p) {
 // Key of a position: its id, or `vocab` (sorts last, ignored by the sums) for padding and ids out of range.  Digits of at
 // most 9 bits from the lowest up; per digit one launch counts every workgroup's positions and a second places them behind
 // all smaller digits and all earlier equal ones.  (Counting the next digit with atomics while the present one is placed
-// saves a launch, but frequent ids meet on one counter: 65 us instead of 10 at 49153 positions.)  Up to 4096 positions are
-// one workgroup's work and all digits one launch.  The sort keeps few CUs busy, so its launches also clear the gradient,
+// saves a launch, but frequent ids meet on one counter: 65 us instead of 10 at 49153 positions.)  Up to 8192 positions are
+// sorted by one workgroup in LDS, all digits in one launch.  The sort keeps few CUs busy, so its launches also clear the gradient,
 // a slice each, with workgroups of their own.
 constexpr int kSortWaves = 16;
 constexpr int kSortThreads = 64 * kSortWaves;
@@ -157,46 +162,70 @@ __device__ __forceinline__ bool clear_slice(const SortParams &p) {
     return true;
 }
 
-// This lane's positions: round r of wave w takes 64 neighbours, waves follow each other.  Past the end: no position.
-template <int R>                             // rounds: positions of a lane, kept in registers
-struct SortItems {
-    int at[R];                               // -1: none
-    uint32_t key[R];
-    __device__ __forceinline__ SortItems(const SortParams &p, int pass) {
-        const long first = (long)blockIdx.x * kSortThreads * R + (threadIdx.x >> 6) * 64 * R + (threadIdx.x & 63);
+// Adds the digits of a wave's lanes to its counts, one atomic for all lanes of a digit (padding would put all 64 on one
+// counter); returns how many of the wave's earlier positions, this round's lower lanes included, have the lane's digit.
+__device__ __forceinline__ uint32_t count_digits(bool live, uint32_t digit, uint32_t *counts, int bits) {
+    const int lane = threadIdx.x & 63;
+    unsigned long long same = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+        const unsigned long long ones = __ballot((digit >> b) & 1u);
+        same &= ((digit >> b) & 1u) ? ones : ~ones;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    uint32_t earlier = 0;
+    if (live && rank == 0) earlier = atomicAdd(counts + digit, (uint32_t)__popcll(same));
+    return __shfl(earlier, same ? __ffsll((long long)same) - 1 : 0, 64) + rank;
+}
+
+// Exclusive sums of total[0 .. bins) in place by one wave, at most eight digits a lane.
+__device__ __forceinline__ void scan_totals(uint32_t *total, int bins) {
+    const int lane = threadIdx.x & 63;
+    uint32_t v[8], s = 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            at[r] = first + 64 * r < p.M ? (int)(first + 64 * r) : -1;
-            key[r] = at[r] >= 0 ? sort_key(p, pass, at[r]) : 0;
-        }
+    for (int j = 0; j < 8; ++j) {
+        v[j] = s;
+        s += lane * 8 + j < bins ? total[lane * 8 + j] : 0;
     }
-    // Adds round r's digits to the wave's counts, one atomic for all lanes of a digit (padding would put all 64 on one
-    // counter); returns how many of the wave's earlier positions, this round's lower lanes included, have the lane's digit.
-    __device__ __forceinline__ uint32_t count(int r, uint32_t *counts, int shift, int bits) const {
-        const int lane = threadIdx.x & 63;
-        const uint32_t digit = (key[r] >> shift) & ((1u << bits) - 1);
-        unsigned long long same = __ballot(at[r] >= 0);
-        for (int b = 0; b < bits; ++b) {
-            const unsigned long long ones = __ballot((digit >> b) & 1u);
-            same &= ((digit >> b) & 1u) ? ones : ~ones;
-        }
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        uint32_t earlier = 0;
-        if (at[r] >= 0 && rank == 0) earlier = atomicAdd(counts + digit, (uint32_t)__popcll(same));
-        return __shfl(earlier, same ? __ffsll((long long)same) - 1 : 0, 64) + rank;
+    uint32_t incl = s;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t o = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += o;
     }
-};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (lane * 8 + j < bins) total[lane * 8 + j] = incl - s + v[j];
+}
+
+// at[wave][d], the waves' counts, become the places of their first positions; total[d]: where the digit's first position of this
+// workgroup goes.  One thread a digit.
+__device__ __forceinline__ void place_waves(uint32_t (&n)[kSortWaves], uint32_t *at, int stride, int d, uint32_t place) {
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+        at[w * stride + d] = place;
+        place += n[w];
+    }
+}
+
+// A lane's positions: round r of wave w takes 64 neighbours, waves follow each other.  -1: past the end.
+template <int R>
+__device__ __forceinline__ int sort_item(const SortParams &p, int r) {
+    const long i = (long)blockIdx.x * kSortThreads * R + (threadIdx.x >> 6) * 64 * R + 64 * r + (threadIdx.x & 63);
+    return i < p.M ? (int)i : -1;
+}
 
 template <int R>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortParams p, int pass) {
     if (clear_slice(p)) return;
     __shared__ uint32_t h[1 << kMaxBits];
     const int bins = 1 << p.bits;
-    const SortItems<R> it(p, pass);
+    uint32_t key[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = sort_item<R>(p, r) >= 0 ? sort_key(p, pass, sort_item<R>(p, r)) : 0;
     if ((int)threadIdx.x < bins) h[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < R; ++r) it.count(r, h, pass * p.bits, p.bits);
+    for (int r = 0; r < R; ++r) count_digits(sort_item<R>(p, r) >= 0, (key[r] >> (pass * p.bits)) & (bins - 1), h, p.bits);
     __syncthreads();
     if ((int)threadIdx.x < bins) p.hist[(long)blockIdx.x * bins + threadIdx.x] = h[threadIdx.x];
 }
@@ -231,82 +260,105 @@ __global__ __launch_bounds__(kSortThreads) void sort_scan_kernel(const SortParam
 }
 
 template <int R>
-__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortParams p, int first_pass, int last_pass) {
+__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortParams p, int pass) {
     if (clear_slice(p)) return;
     __shared__ uint32_t at[kSortWaves][1 << kMaxBits];      // per wave and digit: positions, then the place of the first
     __shared__ uint32_t total[1 << kMaxBits];
-    const int bins = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int bins = 1 << p.bits, wave = threadIdx.x >> 6, shift = pass * p.bits;
     const int d = threadIdx.x;                               // bins <= 512: at most one digit per thread
-    for (int pass = first_pass; pass <= last_pass; ++pass) { // more than one only where there is one workgroup
-        const int shift = pass * p.bits;
-        const SortItems<R> it(p, pass);
+    uint32_t key[R], earlier[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = sort_item<R>(p, r) >= 0 ? sort_key(p, pass, sort_item<R>(p, r)) : 0;
+    for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) at[i >> p.bits][i & (bins - 1)] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) earlier[r] = count_digits(sort_item<R>(p, r) >= 0, (key[r] >> shift) & (bins - 1), at[wave], p.bits);
+    uint32_t before = 0, sum = 0;
+    if (p.totals && d < bins) {
+        before = p.hist[(long)blockIdx.x * bins + d];
+        sum = p.totals[d];
+    } else if (d < bins) {
+        const uint32_t *h = p.hist + d;
+#pragma unroll 16
+        for (int b = 0; b < p.blocks; ++b) {
+            const uint32_t n = h[(long)b * bins];
+            before += b < (int)blockIdx.x ? n : 0;
+            sum += n;
+        }
+    }
+    if (d < bins) total[d] = sum;
+    __syncthreads();
+    uint32_t n[kSortWaves] = {};
+    if (d < bins)
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) n[w] = at[w][d];
+    if (wave == 0) scan_totals(total, bins);
+    __syncthreads();
+    if (d < bins) place_waves(n, at[0], 1 << kMaxBits, d, total[d] + before);
+    __syncthreads();
+    uint32_t *keys_out = p.keys[pass & 1], *pos_out = p.pos[pass & 1];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = sort_item<R>(p, r);
+        if (i < 0) continue;
+        const uint32_t place = at[wave][(key[r] >> shift) & (bins - 1)] + earlier[r];
+        keys_out[place] = key[r];
+        pos_out[place] = pass == 0 ? (uint32_t)i : p.pos[(pass - 1) & 1][i];
+    }
+}
+
+// All digits of up to 8192 positions by one workgroup: key and position of an item in one word (ids below 2^19), which
+// moves through LDS from digit to digit.
+constexpr int kSmallPosBits = 13, kSmallBits = 8;
+template <int R>
+__global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const SortParams p) {
+    if (clear_slice(p)) return;
+    __shared__ uint32_t item[kSortThreads * R];
+    __shared__ uint32_t at[kSortWaves][1 << kSmallBits];
+    __shared__ uint32_t total[1 << kSmallBits];
+    const int bins = 1 << p.bits, wave = threadIdx.x >> 6, d = threadIdx.x;
+    uint32_t v[R], earlier[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = sort_item<R>(p, r);
+        v[r] = i >= 0 ? sort_key(p, 0, i) << kSmallPosBits | (uint32_t)i : 0;
+    }
+    for (int pass = 0; pass < p.passes; ++pass) {
+        const int shift = kSmallPosBits + pass * p.bits;
         for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) at[i >> p.bits][i & (bins - 1)] = 0;
         __syncthreads();
-        uint32_t earlier[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) earlier[r] = it.count(r, at[wave], shift, p.bits);
-        uint32_t before = 0, sum = 0;
-        if (p.totals && d < bins) {
-            before = p.hist[(long)blockIdx.x * bins + d];
-            sum = p.totals[d];
-        } else if (p.blocks > 1 && d < bins) {
-            const uint32_t *h = p.hist + d;
-#pragma unroll 16
-            for (int b = 0; b < p.blocks; ++b) {
-                const uint32_t n = h[(long)b * bins];
-                before += b < (int)blockIdx.x ? n : 0;
-                sum += n;
-            }
-        }
+        for (int r = 0; r < R; ++r) earlier[r] = count_digits(sort_item<R>(p, r) >= 0, (v[r] >> shift) & (bins - 1), at[wave], p.bits);
         __syncthreads();
         uint32_t n[kSortWaves] = {};
         if (d < bins) {
-            uint32_t mine = 0;
+            uint32_t sum = 0;
 #pragma unroll
             for (int w = 0; w < kSortWaves; ++w) {
                 n[w] = at[w][d];
-                mine += n[w];
+                sum += n[w];
             }
-            total[d] = p.blocks > 1 ? sum : mine;
+            total[d] = sum;
         }
         __syncthreads();
-        // exclusive scan of the totals by one wave, eight digits per lane
-        if (wave == 0) {
-            uint32_t v[8], s = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = s;
-                s += lane * 8 + j < bins ? total[lane * 8 + j] : 0;
-            }
-            uint32_t incl = s;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const uint32_t o = __shfl_up(incl, off, 64);
-                if (lane >= off) incl += o;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (lane * 8 + j < bins) total[lane * 8 + j] = incl - s + v[j];
-        }
+        if (wave == 0) scan_totals(total, bins);
         __syncthreads();
-        if (d < bins) {
-            uint32_t place = total[d] + before;
-#pragma unroll
-            for (int w = 0; w < kSortWaves; ++w) {
-                at[w][d] = place;
-                place += n[w];
-            }
-        }
+        if (d < bins) place_waves(n, at[0], 1 << kSmallBits, d, total[d]);
         __syncthreads();
-        uint32_t *keys_out = p.keys[pass & 1], *pos_out = p.pos[pass & 1];
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (it.at[r] >= 0) {
-                const uint32_t place = at[wave][(it.key[r] >> shift) & (bins - 1)] + earlier[r];
-                keys_out[place] = it.key[r];
-                pos_out[place] = pass == 0 ? (uint32_t)it.at[r] : p.pos[(pass - 1) & 1][it.at[r]];
-            }
-        __syncthreads();                                     // the next pass of the same workgroup reads what all its waves wrote
+            if (sort_item<R>(p, r) >= 0) item[at[wave][(v[r] >> shift) & (bins - 1)] + earlier[r]] = v[r];
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (sort_item<R>(p, r) >= 0) v[r] = item[sort_item<R>(p, r)];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = sort_item<R>(p, r);
+        if (i < 0) continue;
+        p.keys[0][i] = v[r] >> kSmallPosBits;
+        p.pos[0][i] = v[r] & ((1u << kSmallPosBits) - 1);
     }
 }
 
@@ -457,21 +509,24 @@ __global__ __launch_bounds__(256) void segment_join_kernel(const SumParams p) {
 }
 
 struct BwdPlan {
+    bool small;
     int rounds, blocks, passes, bits, spans, part_ld;
     size_t keys[2], pos[2], hist, totals, partial, total;
 };
 BwdPlan bwd_plan(long M, long E, long vocab) {
     BwdPlan w{};
     if (M <= kFew) { w.total = 16; return w; }
+    int bits = 0;
+    while ((vocab >> bits) != 0) ++bits;           // keys 0 .. vocab
+    w.small = M <= 1 << kSmallPosBits && bits + kSmallPosBits <= 32;
+    const int most = w.small ? kSmallBits : kMaxBits;
+    w.passes = (bits + most - 1) / most;
+    w.bits = (bits + w.passes - 1) / w.passes;
     // A workgroup scatters its positions line by line, so few of them are dealt to many workgroups: up to 131072 rows 1 round each
     // (65536 rows of 64 into 50000: 38 us, with 4 rounds 49).  Up to kFewBlocks workgroups each sums the counts of the others by
     // itself, which is one launch less; with more of them that grows with the square.
-    w.rounds = M <= 4 * kSortThreads || M > kFewBlocks * kSortThreads ? 4 : 1;
+    w.rounds = w.small ? (M <= 4 * kSortThreads ? 4 : 8) : M > (long)kFewBlocks * kSortThreads ? 4 : 1;
     w.blocks = (int)((M + kSortThreads * w.rounds - 1) / (kSortThreads * w.rounds));
-    int bits = 0;
-    while ((vocab >> bits) != 0) ++bits;           // keys 0 .. vocab
-    w.passes = (bits + kMaxBits - 1) / kMaxBits;
-    w.bits = (bits + w.passes - 1) / w.passes;
     w.spans = (int)((M + kSpan - 1) / kSpan);
     w.part_ld = (int)((E + 3) / 4 * 4);
     size_t off = 0;
@@ -597,7 +652,7 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
         sp.pos[k] = reinterpret_cast<uint32_t *>(ws + w.pos[k]);
     }
     // the launches of the sort clear a slice of the gradient each, 64 KiB and more per workgroup
-    const int launches = w.blocks == 1 ? 1 : 2 * w.passes;
+    const int launches = w.small ? 1 : 2 * w.passes;
     const long cells = accumulate ? 0 : vocab * E;
     int launch = 0;
     auto grid_of = [&]() {
@@ -608,24 +663,27 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
         const long wgs = (sp.clear_to - sp.clear_from + 16383) / 16384;
         return dim3((unsigned)(w.blocks + (wgs < 512 ? wgs : 512)));
     };
-#define TC_SORT(KERNEL, ...)                                                                                    \
+#define TC_SORT(KERNEL)                                                                                         \
     do {                                                                                                        \
         const dim3 grid = grid_of();                                                                            \
-        if (w.rounds == 1) TC_LAUNCH(KERNEL<1>, grid, dim3(kSortThreads), 0, s, sp, __VA_ARGS__);               \
-        else TC_LAUNCH(KERNEL<4>, grid, dim3(kSortThreads), 0, s, sp, __VA_ARGS__);                             \
+        if (w.rounds == 1) TC_LAUNCH(KERNEL<1>, grid, dim3(kSortThreads), 0, s, sp, pass);                      \
+        else TC_LAUNCH(KERNEL<4>, grid, dim3(kSortThreads), 0, s, sp, pass);                                    \
     } while (0)
-    if (w.blocks == 1) {
-        TC_SORT(sort_place_kernel, 0, w.passes - 1);
+    if (w.small) {
+        const dim3 grid = grid_of();
+        if (w.rounds == 4) TC_LAUNCH(sort_small_kernel<4>, grid, dim3(kSortThreads), 0, s, sp);
+        else TC_LAUNCH(sort_small_kernel<8>, grid, dim3(kSortThreads), 0, s, sp);
     } else {
         for (int pass = 0; pass < w.passes; ++pass) {
-            TC_SORT(sort_count_kernel, pass);
+            TC_SORT(sort_count_kernel);
             if (sp.totals) TC_LAUNCH(sort_scan_kernel, dim3((unsigned)(((1 << w.bits) + 63) / 64)), dim3(kSortThreads), 0, s, sp);
-            TC_SORT(sort_place_kernel, pass, pass);
+            TC_SORT(sort_place_kernel);
         }
     }
 #undef TC_SORT
     SumParams q{};
-    q.keys = sp.keys[(w.passes - 1) & 1]; q.pos = sp.pos[(w.passes - 1) & 1];
+    const int sorted = w.small ? 0 : (w.passes - 1) & 1;
+    q.keys = sp.keys[sorted]; q.pos = sp.pos[sorted];
     q.dy = dy; q.ld_dy = ld_dy;
     q.out = d_table;
     q.partial = reinterpret_cast<float *>(ws + w.partial);
