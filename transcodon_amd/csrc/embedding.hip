@@ -162,19 +162,31 @@ __device__ __forceinline__ bool clear_slice(const SortParams &p) {
     return true;
 }
 
-// Adds the digits of a wave's lanes to its counts, one atomic for all lanes of a digit (padding would put all 64 on one
-// counter); returns how many of the wave's earlier positions, this round's lower lanes included, have the lane's digit.
-__device__ __forceinline__ uint32_t count_digits(bool live, uint32_t digit, uint32_t *counts, int bits) {
+// Adds the digits of a wave's lanes, R rounds of them, to its counts, one atomic for all lanes of a digit and round (padding
+// would put all 64 on one counter); earlier[r]: how many of the wave's positions before, in order of rounds and lanes, have
+// the lane's digit.  Three loops, so that the atomics of all rounds are under way together.
+template <int R>
+__device__ __forceinline__ void count_digits(const bool (&live)[R], const uint32_t (&digit)[R], uint32_t *counts, int bits,
+                                             uint32_t (&earlier)[R]) {
     const int lane = threadIdx.x & 63;
-    unsigned long long same = __ballot(live);
-    for (int b = 0; b < bits; ++b) {
-        const unsigned long long ones = __ballot((digit >> b) & 1u);
-        same &= ((digit >> b) & 1u) ? ones : ~ones;
+    unsigned long long same[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        same[r] = __ballot(live[r]);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned long long ones = __ballot((digit[r] >> b) & 1u);
+            same[r] &= ((digit[r] >> b) & 1u) ? ones : ~ones;
+        }
     }
-    const int rank = __popcll(same & ((1ull << lane) - 1));
-    uint32_t earlier = 0;
-    if (live && rank == 0) earlier = atomicAdd(counts + digit, (uint32_t)__popcll(same));
-    return __shfl(earlier, same ? __ffsll((long long)same) - 1 : 0, 64) + rank;
+    uint32_t old[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        old[r] = 0;
+        if (live[r] && (same[r] & ((1ull << lane) - 1)) == 0) old[r] = atomicAdd(counts + digit[r], (uint32_t)__popcll(same[r]));
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        earlier[r] = __shfl(old[r], same[r] ? __ffsll((long long)same[r]) - 1 : 0, 64) + __popcll(same[r] & ((1ull << lane) - 1));
 }
 
 // Exclusive sums of total[0 .. bins) in place by one wave, at most eight digits a lane.
@@ -219,13 +231,18 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortPara
     if (clear_slice(p)) return;
     __shared__ uint32_t h[1 << kMaxBits];
     const int bins = 1 << p.bits;
-    uint32_t key[R];
+    uint32_t key[R], digit[R], earlier[R];
+    bool live[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) key[r] = sort_item<R>(p, r) >= 0 ? sort_key(p, pass, sort_item<R>(p, r)) : 0;
     if ((int)threadIdx.x < bins) h[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < R; ++r) count_digits(sort_item<R>(p, r) >= 0, (key[r] >> (pass * p.bits)) & (bins - 1), h, p.bits);
+    for (int r = 0; r < R; ++r) {
+        live[r] = sort_item<R>(p, r) >= 0;
+        digit[r] = (key[r] >> (pass * p.bits)) & (bins - 1);
+    }
+    count_digits<R>(live, digit, h, p.bits, earlier);
     __syncthreads();
     if ((int)threadIdx.x < bins) p.hist[(long)blockIdx.x * bins + threadIdx.x] = h[threadIdx.x];
 }
@@ -266,13 +283,18 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortPara
     __shared__ uint32_t total[1 << kMaxBits];
     const int bins = 1 << p.bits, wave = threadIdx.x >> 6, shift = pass * p.bits;
     const int d = threadIdx.x;                               // bins <= 512: at most one digit per thread
-    uint32_t key[R], earlier[R];
+    uint32_t key[R], digit[R], earlier[R];
+    bool live[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) key[r] = sort_item<R>(p, r) >= 0 ? sort_key(p, pass, sort_item<R>(p, r)) : 0;
     for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) at[i >> p.bits][i & (bins - 1)] = 0;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < R; ++r) earlier[r] = count_digits(sort_item<R>(p, r) >= 0, (key[r] >> shift) & (bins - 1), at[wave], p.bits);
+    for (int r = 0; r < R; ++r) {
+        live[r] = sort_item<R>(p, r) >= 0;
+        digit[r] = (key[r] >> shift) & (bins - 1);
+    }
+    count_digits<R>(live, digit, at[wave], p.bits, earlier);
     uint32_t before = 0, sum = 0;
     if (p.totals && d < bins) {
         before = p.hist[(long)blockIdx.x * bins + d];
@@ -301,7 +323,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const SortPara
     for (int r = 0; r < R; ++r) {
         const int i = sort_item<R>(p, r);
         if (i < 0) continue;
-        const uint32_t place = at[wave][(key[r] >> shift) & (bins - 1)] + earlier[r];
+        const uint32_t place = at[wave][digit[r]] + earlier[r];
         keys_out[place] = key[r];
         pos_out[place] = pass == 0 ? (uint32_t)i : p.pos[(pass - 1) & 1][i];
     }
@@ -317,10 +339,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const SortPara
     __shared__ uint32_t at[kSortWaves][1 << kSmallBits];
     __shared__ uint32_t total[1 << kSmallBits];
     const int bins = 1 << p.bits, wave = threadIdx.x >> 6, d = threadIdx.x;
-    uint32_t v[R], earlier[R];
+    uint32_t v[R], digit[R], earlier[R];
+    bool live[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int i = sort_item<R>(p, r);
+        live[r] = i >= 0;
         v[r] = i >= 0 ? sort_key(p, 0, i) << kSmallPosBits | (uint32_t)i : 0;
     }
     for (int pass = 0; pass < p.passes; ++pass) {
@@ -328,7 +352,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const SortPara
         for (int i = threadIdx.x; i < kSortWaves * bins; i += kSortThreads) at[i >> p.bits][i & (bins - 1)] = 0;
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < R; ++r) earlier[r] = count_digits(sort_item<R>(p, r) >= 0, (v[r] >> shift) & (bins - 1), at[wave], p.bits);
+        for (int r = 0; r < R; ++r) digit[r] = (v[r] >> shift) & (bins - 1);
+        count_digits<R>(live, digit, at[wave], p.bits, earlier);
         __syncthreads();
         uint32_t n[kSortWaves] = {};
         if (d < bins) {
@@ -347,11 +372,11 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const SortPara
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (sort_item<R>(p, r) >= 0) item[at[wave][(v[r] >> shift) & (bins - 1)] + earlier[r]] = v[r];
+            if (live[r]) item[at[wave][digit[r]] + earlier[r]] = v[r];
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (sort_item<R>(p, r) >= 0) v[r] = item[sort_item<R>(p, r)];
+            if (live[r]) v[r] = item[sort_item<R>(p, r)];
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -363,11 +388,13 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const SortPara
 }
 
 // ---- segmented sum ----------------------------------------------------------------------------------------
-// A workgroup takes kSumWaves pieces of kPiece positions; each wave sums the runs of its piece, and where a run goes on into
-// the next piece the sums are handed over in LDS.  What crosses the workgroup's ends goes to memory, one row at either
+// A workgroup takes kSumWaves pieces of P positions, a span; each wave sums the runs of its piece, and where a run goes on
+// into the next piece the sums are handed over in LDS.  What crosses the workgroup's ends goes to memory, one row at either
 // end, for segment_join_kernel.  HBM bound: 65536 x 768 f32 rows into 10 are 31 us (181 MB, 5.8 TB/s); the sort and the join
-// around it add 14.  Other shapes (4 to 16 waves, pieces of 8 to 32) are within 10 %, none faster.
-constexpr int kSumWaves = 8, kPiece = 32, kSpan = kSumWaves * kPiece;
+// around it add 14.  Pieces of 32, where 4 to 16 waves and pieces of 8 and 16 are within 10 % and none faster.  Up to 8192
+// positions the chip is not full and a wave's time is its piece's: pieces of 8 (sum of 5632 rows of 64: 10.4 -> 4.7 us, of
+// 1024 rows of 768: 13.1 -> 5.4 us).
+constexpr int kSumWaves = 8, kPiece = 32, kSmallPiece = 8;
 struct SumParams {
     const uint32_t *keys, *pos;       // sorted
     const void *dy;
@@ -375,7 +402,7 @@ struct SumParams {
     float *out;                       // [vocab, E]
     float *partial;                   // [spans][2][part_ld]: run from the span before, run into the span after
     int part_ld;
-    int M, E, spans, accumulate;
+    int M, E, span, spans, accumulate;
     uint32_t vocab;
     float scale;
 };
@@ -395,12 +422,12 @@ __device__ __forceinline__ void write_row(const SumParams &p, uint32_t key, int 
     tc_store_row<float, VEC, LOOSE>(dst, v, p.E - col);
 }
 
-template <typename T, bool LOOSE>
+template <typename T, bool LOOSE, int P>
 __global__ __launch_bounds__(64 * kSumWaves) void segment_sum_kernel(const SumParams p) {
     __shared__ float rows[kSumWaves][2][VEC][64];            // [wave][run from before / run into after]
     __shared__ int open[kSumWaves];                          // bit 0: a run comes from before, 1: one goes on, 2: they are the same
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int begin = blockIdx.x * kSpan + wave * kPiece, n = min(kPiece, p.M - begin);      // n <= 0: nothing left
+    const int begin = (blockIdx.x * kSumWaves + wave) * P, n = min(P, p.M - begin);      // n <= 0: nothing left
     const int col = blockIdx.y * 64 * VEC + lane * VEC;
     const bool in = col < p.E;
     int flags = 0, first_key = -1, last_key = -1;
@@ -478,9 +505,9 @@ __global__ __launch_bounds__(256) void segment_join_kernel(const SumParams p) {
     const int lane = threadIdx.x & 63;
     const int c = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (c + 1 >= p.spans) return;
-    const long begin = (long)c * kSpan;
-    const uint32_t key = p.keys[begin + kSpan - 1];
-    if (key == p.vocab || p.keys[begin + kSpan] != key) return;
+    const long begin = (long)c * p.span;
+    const uint32_t key = p.keys[begin + p.span - 1];
+    if (key == p.vocab || p.keys[begin + p.span] != key) return;
     if (begin > 0 && p.keys[begin - 1] == key) return;       // starts earlier
     const int col = blockIdx.y * 64 * VEC + lane * VEC;
     float acc[VEC];
@@ -491,7 +518,7 @@ __global__ __launch_bounds__(256) void segment_join_kernel(const SumParams p) {
     for (int k0 = c + 1; k0 < p.spans; k0 += 64) {
         // the spans that begin inside the run follow each other without a gap
         const int k = k0 + lane;
-        const int n = __popcll(__ballot(k < p.spans && p.keys[(long)min(k, p.spans - 1) * kSpan] == key));
+        const int n = __popcll(__ballot(k < p.spans && p.keys[(long)min(k, p.spans - 1) * p.span] == key));
         constexpr int U = 8;
         for (int i = 0; i < n && in; i += U) {
             float v[U][VEC];
@@ -510,7 +537,7 @@ __global__ __launch_bounds__(256) void segment_join_kernel(const SumParams p) {
 
 struct BwdPlan {
     bool small;
-    int rounds, blocks, passes, bits, spans, part_ld;
+    int rounds, blocks, passes, bits, piece, spans, part_ld;
     size_t keys[2], pos[2], hist, totals, partial, total;
 };
 BwdPlan bwd_plan(long M, long E, long vocab) {
@@ -527,7 +554,8 @@ BwdPlan bwd_plan(long M, long E, long vocab) {
     // itself, which is one launch less; with more of them that grows with the square.
     w.rounds = w.small ? (M <= 4 * kSortThreads ? 4 : 8) : M > (long)kFewBlocks * kSortThreads ? 4 : 1;
     w.blocks = (int)((M + kSortThreads * w.rounds - 1) / (kSortThreads * w.rounds));
-    w.spans = (int)((M + kSpan - 1) / kSpan);
+    w.piece = M <= 8192 ? kSmallPiece : kPiece;
+    w.spans = (int)((M + kSumWaves * w.piece - 1) / (kSumWaves * w.piece));
     w.part_ld = (int)((E + 3) / 4 * 4);
     size_t off = 0;
     auto take = [&](size_t bytes) {
@@ -688,14 +716,17 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
     q.out = d_table;
     q.partial = reinterpret_cast<float *>(ws + w.partial);
     q.part_ld = w.part_ld;
-    q.M = (int)M; q.E = E; q.spans = w.spans;
+    q.M = (int)M; q.E = E; q.span = kSumWaves * w.piece; q.spans = w.spans;
     q.accumulate = accumulate; q.vocab = (uint32_t)vocab; q.scale = scale;
-#define TC_SUM(T, L) segment_sum_kernel<T, L>
-    TC_EMB_T(TC_SUM, dim3((unsigned)w.spans, slabs), 64 * kSumWaves, q);
+#define TC_SUM(T, L) segment_sum_kernel<T, L, kPiece>
+#define TC_SUM_SMALL(T, L) segment_sum_kernel<T, L, kSmallPiece>
+    if (w.piece == kPiece) TC_EMB_T(TC_SUM, dim3((unsigned)w.spans, slabs), 64 * kSumWaves, q);
+    else TC_EMB_T(TC_SUM_SMALL, dim3((unsigned)w.spans, slabs), 64 * kSumWaves, q);
     if (w.spans > 1) {
         if (loose) TC_LAUNCH(segment_join_kernel<true>, dim3((unsigned)(w.spans + 3) / 4, slabs), dim3(256), 0, s, q);
         else TC_LAUNCH(segment_join_kernel<false>, dim3((unsigned)(w.spans + 3) / 4, slabs), dim3(256), 0, s, q);
     }
+#undef TC_SUM_SMALL
 #undef TC_SUM
 #undef TC_FEW8
 #undef TC_FEW4

@@ -6,7 +6,8 @@
 // bf16 on their way into LDS and the product runs on the bf16 matrix cores with f32 accumulators: no rounding but that
 // of the f32 sums.  dY goes to LDS by direct loads; fragments of both are taken with the transposing LDS read.
 // Two kernels: 128 x 128 output tiles for small products and the last rows, 256 x 256 tiles with two wave groups in
-// alternation for large ones.  grid.y splits the rows; the parts are summed by tc_reduce_slabs in a fixed order.
+// alternation for large ones.  grid.y splits the rows; the parts are summed in a fixed order, by tc_reduce_slabs or,
+// where they are many, by tn8_sum_kernel.
 #include "act8.h"
 #include <type_traits>
 
