@@ -736,8 +736,8 @@ int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, const float *
  * Its gradient.  dh (dtype; NULL without the second norm) and dx_out (f32; may be NULL) are the gradients of h and
  * x_out, y, x_out and stats those of the forward pass.  Writes dy (dtype) and dx (f32; may be dx_out where ld_dxo is E) dense, and the f32
  * gradients of the vectors and of the gate [G,E] (d_gate goes with gate; the others may be NULL).  accumulate: bits 0 .. 4 add to
- * d_post_gamma, d_post_beta, d_pre_gamma, d_pre_beta, d_gate instead of overwriting them.  Column sums have a fixed order:
- * the result is the same every time.
+ * d_post_gamma, d_post_beta, d_pre_gamma, d_pre_beta, d_gate instead of overwriting them; no two of these
+ * buffers may overlap.  Column sums have a fixed order: the result is the same every time.
  */
 size_t tc_gated_residual_norm_bwd_workspace_bytes(long M, int E, int G);     /* 0: unsupported shape */
 int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh, const float *dx_out, long ld_dxo, const void *y, long ldy,

@@ -317,3 +317,44 @@ def test_refusals_without_a_gpu():
                 dict(ldy=4)):
         assert bwd(**bad) == -1, bad
     assert bwd(n=need - 1) == -3
+
+
+def test_gradients_that_overlap_are_refused_without_a_gpu():
+    """Two sums into one buffer would lose one of them (one parameter for both norms, say)."""
+    lib, one = _lib.load(), 1 << 12
+    need = lib.tc_gated_residual_norm_bwd_workspace_bytes(4, 8, 2)
+
+    def bwd(d_post_gamma, d_post_beta, d_pre_gamma, d_pre_beta, d_gate):
+        return lib.tc_gated_residual_norm_bwd(0, one, 8, one, 8, one, 8, one, 8, one, one, one, 0, one, 2, 1.0, one, one, one,
+                                              d_post_gamma, d_post_beta, d_gate, d_pre_gamma, d_pre_beta, 31, 4, 8, 0, one, need, None)
+
+    far = [one * 2, one * 3, one * 4, one * 5, one * 6]
+    for a in range(5):
+        for b in range(5):
+            if a == b:
+                continue
+            bad = list(far)
+            bad[a] = bad[b]
+            assert bwd(*bad) == -1, (a, b)
+            bad[a] = bad[b] + 28                                  # the last of eight values
+            assert bwd(*bad) == -1, (a, b)
+    for a in range(4):                                            # into the gate's second row
+        bad = list(far)
+        bad[a] = far[4] + 32
+        assert bwd(*bad) == -1, a
+
+
+@gpu
+def test_backward_refuses_one_buffer_for_two_gradients():
+    c = _on_gpu(_case(6, 16, torch.float32, 0, False))
+    x_out, h, stats = ops.gated_residual_norm(c["y"], c["x"], c["post_gamma"], None, None, c["pre_gamma"])
+    call = lambda into: ops.gated_residual_norm_bwd(c["dh"], c["dx_out"], c["y"], x_out, stats, c["post_gamma"], None, None,
+                                                    c["pre_gamma"], None, into=into)
+    shared = torch.zeros(16, device=DEV)
+    with pytest.raises(_lib.HipLibraryError, match="overlap"):
+        call([shared, None, None, shared, None])
+    with pytest.raises(ValueError):
+        call([shared])
+    next_to = torch.zeros(2, 16, device=DEV)
+    got, fresh = call([next_to[0], None, None, next_to[1], None]), call(None)
+    assert torch.equal(got[2], fresh[2]) and torch.equal(got[5], fresh[5])

@@ -597,6 +597,15 @@ extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh,
         tc_set_error("tc_gated_residual_norm_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
         return TC_ENOSPC;
     }
+    // the sums are added by workgroups of their own: one buffer for two of them would lose one
+    const float *const sums[5] = {d_post_gamma, d_post_beta, d_pre_gamma, d_pre_beta, d_gate};
+    for (int a = 0; a < 5; ++a)
+        for (int b = 0; b < a; ++b) {
+            const uintptr_t from_a = (uintptr_t)sums[a], from_b = (uintptr_t)sums[b];
+            const uintptr_t len_a = (uintptr_t)E * 4 * (a == 4 ? G : 1), len_b = (uintptr_t)E * 4;
+            TC_REQUIRE(!sums[a] || !sums[b] || from_a + len_a <= from_b || from_b + len_b <= from_a,
+                       "tc_gated_residual_norm_bwd: gradients of the vectors overlap");
+        }
     const int g_esz = gate_dtype == TC_BF16 ? 2 : 4;
     const bool loose = !(tc_rows_aligned(y, ldy, esz, VEC) && tc_rows_aligned(x_out, ldx, 4, VEC) && tc_rows_aligned(gate, E, g_esz, VEC) &&
                (!dh || tc_rows_aligned(dh, ld_dh, esz, VEC)) && (!dx_out || tc_rows_aligned(dx_out, ld_dxo, 4, VEC)) &&

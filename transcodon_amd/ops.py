@@ -501,7 +501,8 @@ def gated_residual_norm_bwd(dh, dx_out, y, x_out, stats, post_gamma, post_beta=N
     (dh is None exactly where there is no second norm); y, x_out and stats are those of the forward pass.
 
     Returns (dy, dx, d_post_gamma, d_post_beta, d_gate, d_pre_gamma, d_pre_beta), f32 but for dy, None where there is no such
-    vector.  into: five f32 buffers or None in the order of the last five, which are added to instead.
+    vector.  into: five f32 buffers or None in the order of the last five, which are added to instead; no two
+    may overlap.
     tc_gated_residual_norm_bwd."""
     dev = _same_device(dh, dx_out, y, x_out, stats, post_gamma, post_beta, gate, pre_gamma, pre_beta, *(into or ()))
     dt, ldy, ldx = _dt(y), _rows(y, "y"), _rows(x_out, "x_out")
@@ -523,6 +524,8 @@ def gated_residual_norm_bwd(dh, dx_out, y, x_out, stats, post_gamma, post_beta=N
     dy = torch.empty(M, E, dtype=y.dtype, device=dev)
     dx = torch.empty(M, E, dtype=torch.float32, device=dev)
     vectors = (post_gamma, post_beta, gate, pre_gamma, pre_beta)
+    if into is not None and len(into) != len(vectors):
+        raise ValueError(f"into has {len(into)} buffers, expected {len(vectors)}")
     empty = torch.empty if M and E else torch.zeros
     # one allocation for the gradients of length E
     fresh = iter(empty(4, E, dtype=torch.float32, device=dev).unbind(0))
