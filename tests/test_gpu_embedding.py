@@ -205,3 +205,13 @@ def test_refusals_without_a_gpu():
     assert bwd(n=need - 1) == -3
     with pytest.raises(_lib.HipLibraryError):
         ops.embedding(torch.zeros(4, dtype=torch.int64), torch.zeros(3, 8))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [100, 600])
+def test_rows_without_a_position_are_zeros_for_any_scale(rows):
+    tok = torch.full((rows,), 3, device=DEV)
+    got = ops.embedding_bwd(tok, torch.ones(rows, 8, device=DEV), 6, scale=float("inf"))
+    want = torch.zeros(6, 8, device=DEV)
+    want[3] = float("inf")
+    assert torch.equal(got, want)

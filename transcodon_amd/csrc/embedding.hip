@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void few_positions_kernel(const FewParams p) {
         for (int j = 0; j < VEC; ++j) old[j] = 0.f;
         if (p.accumulate) tc_load_row<float, VEC, LOOSE>(dst, old, p.E - col);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] = old[j] + p.scale * acc[j];
+        for (int j = 0; j < VEC; ++j) acc[j] = any ? old[j] + p.scale * acc[j] : 0.f;      // zero for any scale
         tc_store_row<float, VEC, LOOSE>(dst, acc, p.E - col);
     }
 }
