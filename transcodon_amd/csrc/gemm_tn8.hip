@@ -463,6 +463,7 @@ Tn8Plan tn8_plan(long M, long ld_dy, int N, int K) {
     const long large = (long)((N + 255) / 256) * ((K + 255) / 256), small = (long)((N + 127) / 128) * ((K + 127) / 128);
     auto parts = [&](long slabs) { return slabs > 1 ? 4000 + slabs * N * K * 8 / 6500 : 0; };
     for (long s = 1; s <= 256; s += s < 16 ? 1 : s < 64 ? 4 : 16) {
+        if (s >= kManySlabs && (long)N * K > (1L << 29)) break;      // tn8_sum_kernel's launch holds fewer than 2^32 threads
         if (s <= nk) {
             const long wgs = small * s;
             const long ns = 2000 + (nk + s - 1) / s * (400 + 600 * (wgs > 256 ? wgs : 256) / 256) + parts(s);
