@@ -358,3 +358,52 @@ def test_backward_refuses_one_buffer_for_two_gradients():
     next_to = torch.zeros(2, 16, device=DEV)
     got, fresh = call([next_to[0], None, None, next_to[1], None]), call(None)
     assert torch.equal(got[2], fresh[2]) and torch.equal(got[5], fresh[5])
+
+
+@gpu
+@pytest.mark.parametrize("E", [3, 6, 300, 515, 766, 768, 1022, 1030, 2048, 2053, 4096, 4098, 8000, 8190, 8192])
+@pytest.mark.parametrize("second", [True, False])
+def test_results_in_place_of_the_residual_stream(E, second):
+    """x_out may be x, and dx may be dx_out: a row's last columns may be read by two lanes, in two waves."""
+    M, lib = 700, _lib.load()
+    c = _on_gpu(_case(M, E, torch.bfloat16, 7, False))
+    pre = (c["pre_gamma"], c["pre_beta"]) if second else (None, None)
+    dh = c["dh"] if second else None
+    P = lambda t: None if t is None else t.data_ptr()
+    stream = torch.cuda.current_stream().cuda_stream
+    x_out, h, stats = ops.gated_residual_norm(c["y"], c["x"], c["post_gamma"], c["post_beta"], c["gate"], *pre, res_scale=0.5)
+    want = ops.gated_residual_norm_bwd(dh, c["dx_out"], c["y"], x_out, stats, c["post_gamma"], c["post_beta"], c["gate"], *pre,
+                                       res_scale=0.5)
+    need = lib.tc_gated_residual_norm_bwd_workspace_bytes(M, E, 7)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    for _ in range(3):
+        x, d, h2, stats2, dy = c["x"].clone(), c["dx_out"].clone(), torch.empty_like(c["y"]), torch.empty_like(stats), torch.empty_like(c["y"])
+        assert lib.tc_gated_residual_norm_fwd(1, P(c["y"]), E, P(x), E, P(c["post_gamma"]), P(c["post_beta"]), 0, P(c["gate"]), 7, 0.5, P(pre[0]),
+                                              P(pre[1]), P(x), P(h2) if second else None, P(stats2), M, E, 0, 1e-5, 1e-5, stream) == 0
+        assert torch.equal(x, x_out) and torch.equal(stats2, stats) and (not second or torch.equal(h2, h))
+        grads = [torch.empty_like(t) for t in want[2:] if t is not None]
+        g = grads + [None] * (5 - len(grads))
+        assert lib.tc_gated_residual_norm_bwd(1, P(dh), E, P(d), E, P(c["y"]), E, P(x_out), E, P(stats), P(c["post_gamma"]), P(c["post_beta"]), 0,
+                                              P(c["gate"]), 7, 0.5, P(pre[0]), P(dy), P(d), P(g[0]), P(g[1]), P(g[2]), P(g[3]), P(g[4]), 0, M, E, 0,
+                                              P(ws), need, stream) == 0
+        for a, b in zip([dy, d, *grads], [t for t in want if t is not None]):
+            assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("E", [1, 2, 3, 5, 257, 513, 769, 1025, 2049, 4097, 8191])
+@pytest.mark.parametrize("G", [0, 1, 5, 40])
+def test_a_row_end_behind_the_last_whole_piece(E, G):
+    """The columns that two lanes hold count once in every sum; the rows next to the result are left as they were."""
+    c = _case(40, E, torch.float32, G, False)
+    g = _on_gpu(c)
+    x_out, h, stats = ops.gated_residual_norm(g["y"], g["x"], g["post_gamma"], g["post_beta"], g["gate"], g["pre_gamma"], g["pre_beta"])
+    got = ops.gated_residual_norm_bwd(g["dh"], g["dx_out"], g["y"], x_out, stats, g["post_gamma"], g["post_beta"], g["gate"], g["pre_gamma"],
+                                      g["pre_beta"])
+    into = [None if t is None else torch.ones_like(t) for t in got[2:]]
+    again = ops.gated_residual_norm_bwd(g["dh"], g["dx_out"], g["y"], x_out, stats, g["post_gamma"], g["post_beta"], g["gate"], g["pre_gamma"],
+                                        g["pre_beta"], into=into)
+    for a, b in zip(got[2:], again[2:]):
+        assert a is None and b is None or torch.equal(a + 1.0, b)
+    # a gradient of beta is a plain sum over the rows of dh: 40 values of size up to 4, f32
+    assert float((got[6].double().cpu() - c["dh"].double().sum(0)).abs().max()) <= 40 * 4 * 40 * 2.0 ** -24

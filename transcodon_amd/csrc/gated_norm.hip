@@ -8,12 +8,11 @@
 // stream and all arithmetic are f32; y, h and their gradients are f32 or bf16.
 //
 // A team of W waves owns a row at a time and keeps it in registers, so every operand is read from memory once; deviations are
-// summed after the mean is known.  HBM bound: 65536 x 768 in bf16 with 64 gate rows 115 us forward (604 MB, 5.3 TB/s; a
-// large copy: 4.9) and 194 us backward (907 MB, 4.7 TB/s).  The backward pass gives each team a run of
+// summed after the mean is known.  HBM bound: 65536 x 768 in bf16 with 64 gate rows 109 us forward (604 MB, 5.5 TB/s; a
+// large copy: 4.9) and 188 us backward (907 MB, 4.8 TB/s).  The backward pass gives each team a run of
 // neighbouring rows and keeps the column sums (gradients of the norms' vectors and of the gate) in registers; teams of
 // a workgroup are added in LDS, workgroups by a second kernel, always in the same order.
 #include "row_io.h"
-#include <math.h>
 
 namespace {
 
@@ -44,17 +43,35 @@ struct Team {                                // W waves that work on one row
     }
 };
 
+// The columns of a lane, NC pieces of VEC.  Every piece has VEC columns of the row: one that would pass its end is moved back, to
+// columns that other lanes have as well.  Those come to the same values, so they may be stored twice, but a sum counts a piece's
+// columns from `skip` on only.  So loads and stores stand in no branch: where paths with different numbers of them meet, the
+// compiler waits for all that are under way (8192 x 4098 bf16 forward: 160 us with the row's end in a branch of its own, 92 so).
+template <bool LOOSE, int W, int NC, int VEC>
+struct Pieces {
+    int col[NC], skip[NC];
+    __device__ __forceinline__ Pieces(int wave, int E) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int want = ((wave + c * W) * 64 + (int)(threadIdx.x & 63)) * VEC;
+            col[c] = min(want, E - VEC);
+            skip[c] = want - col[c];
+        }
+    }
+    __device__ __forceinline__ bool counts(int c, int j) const { return LOOSE ? j >= skip[c] : skip[c] == 0; }
+};
+
 // mean and 1 / sqrt(variance + eps) of a row held as v[NC][VEC]
-template <int W, int NC>
-__device__ __forceinline__ void row_stats(Team<W> &team, const float (&v)[NC][VEC], const int (&n)[NC], int E, int rms, float eps,
-                                          float &mean, float &rstd) {
+template <bool LOOSE, int W, int NC, int VEC>
+__device__ __forceinline__ void row_stats(Team<W> &team, const Pieces<LOOSE, W, NC, VEC> &at, const float (&v)[NC][VEC], int E, int rms,
+                                          float eps, float &mean, float &rstd) {
     mean = 0.f;
     if (!rms) {
         float s = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s += v[c][j];          // zero past the end of the row
+            for (int j = 0; j < VEC; ++j) s += at.counts(c, j) ? v[c][j] : 0.f;
         mean = team.sum(s) / (float)E;
     }
     float q = 0.f;
@@ -62,10 +79,19 @@ __device__ __forceinline__ void row_stats(Team<W> &team, const float (&v)[NC][VE
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            const float d = j < n[c] ? v[c][j] - mean : 0.f;
+            const float d = at.counts(c, j) ? v[c][j] - mean : 0.f;
             q += d * d;
         }
     rstd = rsqrtf(team.sum(q) / (float)E + eps);
+}
+
+// Has the loads that v came from arrive here.
+template <int NC, int VEC>
+__device__ __forceinline__ void arrived(float (&v)[NC][VEC]) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) asm volatile("" : "+v"(v[c][j]));
 }
 
 struct NormParams {
@@ -88,22 +114,40 @@ struct NormParams {
     int teams, rows_per_team, teams_per_group;
 };
 
-template <typename T, typename TG, bool LOOSE, int W, int NC>
+template <typename T, typename TG, bool LOOSE, int W, int NC, int VEC>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_kernel(const NormParams p) {
     __shared__ float red[2][2][W];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Team<W> team{red, W == 1 ? 0 : wave};
     constexpr int kTeams = W == 1 ? 4 : 1;
-    const int col0 = ((W == 1 ? 0 : wave) * 64 + lane) * VEC;
-    int n[NC];                               // values of each piece that the row has
+    const Pieces<LOOSE, W, NC, VEC> at(W == 1 ? 0 : wave, p.E);
+    // One or two teams of many waves fill a CU and meet at barriers: they ask for their next row before they work on this one and
+    // keep the vectors, which are more bytes than a row (8192 x 8192 bf16: 183 -> 157 us, 4096 wide 96 -> 79).  Smaller teams
+    // find others to hide their loads behind.
+    constexpr bool kAhead = W > 4;
+    struct Vectors {
+        float g1[NC][VEC], b1[NC][VEC], gate[NC][VEC], g2[NC][VEC], b2[NC][VEC];
+    } k;
+    auto load_vectors = [&]() {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int left = p.E - (col0 + c * 64 * W * VEC);
-        n[c] = LOOSE ? max(0, min(VEC, left)) : left > 0 ? VEC : 0;
-    }
-    // Two teams of 16 waves fill a CU and meet at barriers: they ask for their next row before they work on this one (4096 x
-    // 8192 bf16: 139 -> 117 us).  Smaller teams find others to hide their loads behind (8192 x 4096: 90 us, asking ahead 93).
-    constexpr bool kAhead = W == 16;
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) k.b1[c][j] = k.g2[c][j] = k.b2[c][j] = 0.f;
+            tc_load_row<float, VEC, LOOSE>(p.g1 + at.col[c], k.g1[c]);
+            if (p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + at.col[c], k.b1[c]);
+            if (p.g2) tc_load_row<float, VEC, LOOSE>(p.g2 + at.col[c], k.g2[c]);
+            if (p.b2) tc_load_row<float, VEC, LOOSE>(p.b2 + at.col[c], k.b2[c]);
+        }
+    };
+    auto load_gate = [&](long row) {
+        const long gate_row = (long)((unsigned)row / (unsigned)p.rows_per_gate) * p.E;      // rows are below 2^31
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) k.gate[c][j] = 1.f;
+            if (p.gate) tc_load_row<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + gate_row + at.col[c], k.gate[c]);
+        }
+    };
     struct Row {
         typename TcRaw<T, VEC>::type y[NC];
         typename TcRaw<float, VEC>::type x[NC];
@@ -111,20 +155,19 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_kernel(const
     auto request = [&](long row) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = col0 + c * 64 * W * VEC;
-            if (n[c] == 0) continue;
-            next.y[c] = tc_raw_load<T, VEC, LOOSE>(static_cast<const T *>(p.y) + row * p.ldy + col, n[c]);
-            next.x[c] = tc_raw_load<float, VEC, LOOSE>(p.x + row * p.ldx + col, n[c]);
+            next.y[c] = tc_raw_load<T, VEC, LOOSE>(static_cast<const T *>(p.y) + row * p.ldy + at.col[c]);
+            next.x[c] = tc_raw_load<float, VEC, LOOSE>(p.x + row * p.ldx + at.col[c]);
         }
     };
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        next.y[c] = typename TcRaw<T, VEC>::type{};
-        next.x[c] = typename TcRaw<float, VEC>::type{};
-    }
     const long step = (long)gridDim.x * kTeams;
     long row = (long)blockIdx.x * kTeams + (W == 1 ? wave : 0);
-    if (kAhead && row < p.M) request(row);
+    if (kAhead && row < p.M) {
+        load_vectors();
+        request(row);
+        arrived(k.g1); arrived(k.b1); arrived(k.g2); arrived(k.b2);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) asm volatile("" : "+v"(next.y[c]), "+v"(next.x[c]));
+    }
     for (; row < p.M; row += step) {
         if (!kAhead) request(row);
         float yv[NC][VEC], xv[NC][VEC];
@@ -133,46 +176,30 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_kernel(const
             tc_raw_widen<T, VEC>(next.y[c], yv[c]);
             tc_raw_widen<float, VEC>(next.x[c], xv[c]);
         }
-        if (kAhead && row + step < p.M) request(row + step);
+        if (!kAhead) load_vectors();
+        load_gate(row);
+        if (kAhead) request(row + step < p.M ? row + step : row);
+        if (W > 1) arrived(xv);                  // x_out may be x: before the team's next barrier, which is before its stores
         float mean1, rstd1;
-        row_stats<W, NC>(team, yv, n, p.E, p.rms, p.eps1, mean1, rstd1);
-        const long gate_row = (long)((unsigned)row / (unsigned)p.rows_per_gate) * p.E;      // rows are below 2^31
+        row_stats(team, at, yv, p.E, p.rms, p.eps1, mean1, rstd1);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = col0 + c * 64 * W * VEC;
-            if (n[c] == 0) continue;
-            float g[VEC], b[VEC], gt[VEC];
-            tc_load_row<float, VEC, LOOSE>(p.g1 + col, g, n[c]);
-            if (p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + col, b, n[c]);
-            if (p.gate) tc_load_row<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + gate_row + col, gt, n[c]);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                float t = (yv[c][j] - mean1) * rstd1 * g[j];
-                if (p.b1) t += b[j];
-                if (p.gate) t *= gt[j];
-                xv[c][j] = p.res_scale * xv[c][j] + t;
-            }
-            tc_store_row<float, VEC, LOOSE>(p.x_out + row * p.E + col, xv[c], n[c]);
+            for (int j = 0; j < VEC; ++j)
+                xv[c][j] = p.res_scale * xv[c][j] + ((yv[c][j] - mean1) * rstd1 * k.g1[c][j] + k.b1[c][j]) * k.gate[c][j];
+            tc_store_row<float, VEC, LOOSE>(p.x_out + row * p.E + at.col[c], xv[c]);
         }
         float mean2 = 0.f, rstd2 = 0.f;
         if (p.g2) {
-            row_stats<W, NC>(team, xv, n, p.E, p.rms, p.eps2, mean2, rstd2);
+            row_stats(team, at, xv, p.E, p.rms, p.eps2, mean2, rstd2);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const int col = col0 + c * 64 * W * VEC;
-                if (n[c] == 0) continue;
-                float g[VEC], b[VEC];
-                tc_load_row<float, VEC, LOOSE>(p.g2 + col, g, n[c]);
-                if (p.b2) tc_load_row<float, VEC, LOOSE>(p.b2 + col, b, n[c]);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    xv[c][j] = (xv[c][j] - mean2) * rstd2 * g[j];
-                    if (p.b2) xv[c][j] += b[j];
-                }
-                tc_store_row<T, VEC, LOOSE>(static_cast<T *>(p.h) + row * p.E + col, xv[c], n[c]);
+                for (int j = 0; j < VEC; ++j) xv[c][j] = (xv[c][j] - mean2) * rstd2 * k.g2[c][j] + k.b2[c][j];
+                tc_store_row<T, VEC, LOOSE>(static_cast<T *>(p.h) + row * p.E + at.col[c], xv[c]);
             }
         }
-        if (p.stats && col0 == 0) *reinterpret_cast<f32x4 *>(p.stats + row * 4) = f32x4{mean1, rstd1, mean2, rstd2};
+        if (p.stats && (W == 1 ? threadIdx.x & 63 : threadIdx.x) == 0) *reinterpret_cast<f32x4 *>(p.stats + row * 4) = f32x4{mean1, rstd1, mean2, rstd2};
     }
 }
 
@@ -181,21 +208,15 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_kernel(const
 //   y^ = (y - mean1) rstd1        dn = D o gate     dy = rstd1 (q - mean(q) - y^ mean(q y^)),  q = dn o g1
 //   dx = res_scale D    d_gate = sum D o n    d_g1 = sum dn o y^   d_b1 = sum dn   d_g2 = sum dh o x^   d_b2 = sum dh
 // (root-mean-square norms: without the mean(p), mean(q) terms).
-template <typename T, typename TG, bool LOOSE, int W, int NC>
+template <typename T, typename TG, bool LOOSE, int W, int NC, int VEC>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(const NormParams p) {
     extern __shared__ float sums[];          // [team][E] (W == 1)
     __shared__ float red[2][2][W];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Team<W> team{red, W == 1 ? 0 : wave};
     constexpr int kTeams = W == 1 ? 4 : 1;   // teams of a workgroup
     const int t = blockIdx.x * kTeams + (W == 1 ? wave : 0);
-    const int col0 = ((W == 1 ? 0 : wave) * 64 + lane) * VEC;
-    int n[NC];                               // values of each piece that the row has
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int left = p.E - (col0 + c * 64 * W * VEC);
-        n[c] = LOOSE ? max(0, min(VEC, left)) : left > 0 ? VEC : 0;
-    }
+    const Pieces<LOOSE, W, NC, VEC> at(W == 1 ? 0 : wave, p.E);
     float acc[4][NC][VEC], dgt[NC][VEC];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -218,46 +239,63 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
     const float inv_e = 1.0f / (float)p.E;
     // A row's operands as they were loaded.  The next row is requested before this one is worked on, since three dependent
     // row reductions leave a wave idle otherwise, and the vectors stay in registers, the gate's row until its group ends
-    // (loading them again for every row: 65536 x 768 bf16 208 instead of 194 us).  Sixteen waves leave 128 registers each,
-    // which hold neither.
-    constexpr bool kAhead = W < 16, kKeep = W < 16;
+    // (loading them again for every row: 65536 x 768 bf16 208 instead of 194 us).  More than eight waves leave too few registers
+    // for either.
+    // No load or store of the loop stands in a branch but those of a new gate row: an operand that is not there is read from one
+    // row of another, and what is loaded before the loop is waited for there.
+    constexpr bool kAhead = W <= 8, kKeep = W <= 8;
+    const T *const dh_rows = p.g2 ? static_cast<const T *>(p.dh) : static_cast<const T *>(p.y);
+    const float *const d_rows = p.dx_out ? p.dx_out : p.x;
+    const long ldx = p.g2 ? p.ldx : 0, ld_dh = p.g2 ? p.ld_dh : 0, ld_d = p.dx_out ? p.ld_dxo : 0;
     struct Row {
         typename TcRaw<T, VEC>::type y[NC], dh[NC];
         typename TcRaw<float, VEC>::type x[NC], d[NC];
+        typename TcRaw<TG, VEC>::type gate[NC];
         f32x4 st;
     } next;
+    auto gate_row_of = [&](long row) { return (long)((unsigned)row / (unsigned)p.rows_per_gate) * p.E; };      // rows are below 2^31
+    long kept_gate = -1;                     // the row of the gate that `next` or kgt holds
+    bool fresh_gate = false;
     auto request = [&](long row) {
+        if (kKeep && p.gate) {
+            fresh_gate = gate_row_of(row) != kept_gate;
+            if (fresh_gate) {
+                kept_gate = gate_row_of(row);
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+                    next.gate[c] = tc_raw_load<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + kept_gate + at.col[c]);
+            }
+        }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = col0 + c * 64 * W * VEC;
-            if (n[c] == 0) continue;
-            next.y[c] = tc_raw_load<T, VEC, LOOSE>(static_cast<const T *>(p.y) + row * p.ldy + col, n[c]);
-            if (p.g2) {
-                next.x[c] = tc_raw_load<float, VEC, LOOSE>(p.x + row * p.ldx + col, n[c]);
-                next.dh[c] = tc_raw_load<T, VEC, LOOSE>(static_cast<const T *>(p.dh) + row * p.ld_dh + col, n[c]);
-            }
-            if (p.dx_out) next.d[c] = tc_raw_load<float, VEC, LOOSE>(p.dx_out + row * p.ld_dxo + col, n[c]);
+            next.y[c] = tc_raw_load<T, VEC, LOOSE>(static_cast<const T *>(p.y) + row * p.ldy + at.col[c]);
+            next.x[c] = tc_raw_load<float, VEC, LOOSE>(p.x + row * ldx + at.col[c]);
+            next.dh[c] = tc_raw_load<T, VEC, LOOSE>(dh_rows + row * ld_dh + at.col[c]);
+            next.d[c] = tc_raw_load<float, VEC, LOOSE>(d_rows + row * ld_d + at.col[c]);
         }
         next.st = *reinterpret_cast<const f32x4 *>(p.stats + row * 4);
     };
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        next.y[c] = next.dh[c] = typename TcRaw<T, VEC>::type{};
-        next.x[c] = next.d[c] = typename TcRaw<float, VEC>::type{};
-    }
     float kg1[NC][VEC], kb1[NC][VEC], kg2[NC][VEC], kgt[NC][VEC];
-    long kept_gate = -1;
     if (kKeep) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = col0 + c * 64 * W * VEC;
-            if (n[c] == 0) continue;
-            tc_load_row<float, VEC, LOOSE>(p.g1 + col, kg1[c], n[c]);
-            if (p.gate && p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + col, kb1[c], n[c]);
-            if (p.g2) tc_load_row<float, VEC, LOOSE>(p.g2 + col, kg2[c], n[c]);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                kb1[c][j] = kg2[c][j] = 0.f;
+                kgt[c][j] = 1.f;
+            }
+            tc_load_row<float, VEC, LOOSE>(p.g1 + at.col[c], kg1[c]);
+            if (p.gate && p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + at.col[c], kb1[c]);
+            if (p.g2) tc_load_row<float, VEC, LOOSE>(p.g2 + at.col[c], kg2[c]);
         }
     }
-    if (kAhead && begin < end) request(begin);
+    if (kAhead && begin < end) {
+        request(begin);
+        arrived(kg1); arrived(kb1); arrived(kg2);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) asm volatile("" : "+v"(next.y[c]), "+v"(next.x[c]), "+v"(next.dh[c]), "+v"(next.d[c]));
+        asm volatile("" : "+v"(next.st));
+    }
     for (long row = begin; row < end; ++row) {
         if (!kAhead) request(row);
         float yv[NC][VEC], xv[NC][VEC], dh[NC][VEC], d[NC][VEC];
@@ -267,17 +305,27 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
             tc_raw_widen<float, VEC>(next.x[c], xv[c]);
             tc_raw_widen<T, VEC>(next.dh[c], dh[c]);
             tc_raw_widen<float, VEC>(next.d[c], d[c]);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) d[c][j] = p.dx_out ? d[c][j] : 0.f;
         }
         const f32x4 st = next.st;
-        if (kAhead && row + 1 < end) request(row + 1);
+        if (kKeep && fresh_gate) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) tc_raw_widen<TG, VEC>(next.gate[c], kgt[c]);
+            arrived(kgt);
+        }
+        if (kAhead) request(min(row + 1, end - 1));
+        // dx may be dx_out: every wave has its values of that before the barrier that is before the stores
+        if (W > 1 && kAhead) {
+            arrived(d);
+            if (!p.g2) __syncthreads();
+        }
         if (p.g2) {
             float s1 = 0.f, s2 = 0.f;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const int col = col0 + c * 64 * W * VEC;
-                if (n[c] == 0) continue;
                 float g[VEC];
-                if (!kKeep) tc_load_row<float, VEC, LOOSE>(p.g2 + col, g, n[c]);
+                if (!kKeep) tc_load_row<float, VEC, LOOSE>(p.g2 + at.col[c], g);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     if (kKeep) g[j] = kg2[c][j];
@@ -285,8 +333,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
                     acc[2][c][j] += dh[c][j] * xh;
                     acc[3][c][j] += dh[c][j];
                     const float q = dh[c][j] * g[j];
-                    s1 += q;
-                    s2 += q * xh;
+                    const float counted = at.counts(c, j) ? q : 0.f;
+                    s1 += counted;
+                    s2 += counted * xh;
                     xv[c][j] = xh;
                     dh[c][j] = q;
                 }
@@ -298,72 +347,70 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) d[c][j] += st[3] * (dh[c][j] - m1 - xv[c][j] * m2);
         }
-        const long gate_row = (long)((unsigned)row / (unsigned)p.rows_per_gate) * p.E;      // rows are below 2^31
-        if (kKeep && p.gate && gate_row != kept_gate) {
-            kept_gate = gate_row;
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-                if (n[c] > 0)
-                    tc_load_row<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + gate_row + col0 + c * 64 * W * VEC, kgt[c], n[c]);
+        if (!kAhead) {                       // a barrier of its own, where registers are too few to have the values early
+            arrived(d);
+            __syncthreads();
         }
+        const long gate_row = gate_row_of(row);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = col0 + c * 64 * W * VEC;
-            if (n[c] == 0) continue;
             float g[VEC], b[VEC], gt[VEC], o[VEC];
             if (!kKeep) {
-                tc_load_row<float, VEC, LOOSE>(p.g1 + col, g, n[c]);
-                if (p.gate) tc_load_row<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + gate_row + col, gt, n[c]);
-                if (p.gate && p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + col, b, n[c]);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    b[j] = 0.f;
+                    gt[j] = 1.f;
+                }
+                tc_load_row<float, VEC, LOOSE>(p.g1 + at.col[c], g);
+                if (p.gate) tc_load_row<TG, VEC, LOOSE>(static_cast<const TG *>(p.gate) + gate_row + at.col[c], gt);
+                if (p.gate && p.b1) tc_load_row<float, VEC, LOOSE>(p.b1 + at.col[c], b);
             }
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 if (kKeep) { g[j] = kg1[c][j]; b[j] = kb1[c][j]; gt[j] = kgt[c][j]; }
                 const float yh = (yv[c][j] - st[0]) * st[1];
-                float dn = d[c][j];
-                if (p.gate) {
-                    float t = yh * g[j];
-                    if (p.b1) t += b[j];
-                    dgt[c][j] += dn * t;
-                    dn *= gt[j];
-                }
+                dgt[c][j] += d[c][j] * (yh * g[j] + b[j]);
+                const float dn = d[c][j] * gt[j];
                 acc[0][c][j] += dn * yh;
                 acc[1][c][j] += dn;
                 const float q = dn * g[j];
-                s1 += q;
-                s2 += q * yh;
+                const float counted = at.counts(c, j) ? q : 0.f;
+                s1 += counted;
+                s2 += counted * yh;
                 o[j] = p.res_scale * d[c][j];
                 yv[c][j] = yh;
                 d[c][j] = q;
             }
-            tc_store_row<float, VEC, LOOSE>(p.dx + row * p.E + col, o, n[c]);
+            tc_store_row<float, VEC, LOOSE>(p.dx + row * p.E + at.col[c], o);
         }
         team.sum2(s1, s2);
         const float m1 = p.rms ? 0.f : s1 * inv_e, m2 = s2 * inv_e;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = col0 + c * 64 * W * VEC;
-            if (n[c] == 0) continue;
             float o[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) o[j] = st[1] * (d[c][j] - m1 - yv[c][j] * m2);
-            tc_store_row<T, VEC, LOOSE>(static_cast<T *>(p.dy) + row * p.E + col, o, n[c]);
+            tc_store_row<T, VEC, LOOSE>(static_cast<T *>(p.dy) + row * p.E + at.col[c], o);
         }
         // the team's last row of a gate group: the group's gradient, or this team's part of it
         if (p.gate && p.teams_per_group == 0 && ((unsigned)row + 1) % (unsigned)p.rows_per_gate == 0) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const int col = col0 + c * 64 * W * VEC;
-                if (n[c] == 0) continue;
-                float *to = p.d_gate + gate_row + col;
-                if (p.accumulate & 16) {
+                float *to = p.d_gate + gate_row + at.col[c];
+                if (at.skip[c] == 0) {
                     float old[VEC];
-                    tc_load_row<float, VEC, LOOSE>(to, old, n[c]);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) dgt[c][j] += old[j];
+                    for (int j = 0; j < VEC; ++j) old[j] = 0.f;
+                    if (p.accumulate & 16) tc_load_row<float, VEC, LOOSE>(to, old);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) old[j] += dgt[c][j];
+                    tc_store_row<float, VEC, LOOSE>(to, old);
+                } else if (LOOSE) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        if (j >= at.skip[c]) to[j] = p.accumulate & 16 ? to[j] + dgt[c][j] : dgt[c][j];
                 }
-                tc_store_row<float, VEC, LOOSE>(to, dgt[c], n[c]);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) dgt[c][j] = 0.f;
             }
@@ -373,22 +420,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
     if (p.gate && p.teams_per_group > 0 && t < p.teams) {
         float *to = p.ws + (long)gridDim.x * 4 * p.E + (long)t * p.E;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int col = col0 + c * 64 * W * VEC;
-            if (n[c] > 0) tc_store_row<float, VEC, LOOSE>(to + col, dgt[c], n[c]);
-        }
+        for (int c = 0; c < NC; ++c) tc_store_row<float, VEC, LOOSE>(to + at.col[c], dgt[c]);
     }
     float *to = p.ws + (long)blockIdx.x * 4 * p.E;
     if constexpr (W == 1) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int col = col0 + c * 64 * VEC;
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
-                    if (j < n[c]) sums[wave * p.E + col + j] = acc[v][c][j];
-            }
+                    if (at.counts(c, j)) sums[wave * p.E + at.col[c] + j] = acc[v][c][j];
             __syncthreads();
             for (int i = threadIdx.x; i < p.E; i += 256) to[v * p.E + i] = (sums[i] + sums[p.E + i]) + (sums[2 * p.E + i] + sums[3 * p.E + i]);
             __syncthreads();
@@ -397,10 +439,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_bwd_kernel(c
 #pragma unroll
         for (int v = 0; v < 4; ++v)
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int col = col0 + c * 64 * W * VEC;
-                if (n[c] > 0) tc_store_row<float, VEC, LOOSE>(to + (long)v * p.E + col, acc[v][c], n[c]);
-            }
+            for (int c = 0; c < NC; ++c) tc_store_row<float, VEC, LOOSE>(to + (long)v * p.E + at.col[c], acc[v][c]);
     }
 }
 
@@ -432,20 +471,28 @@ __global__ __launch_bounds__(1024) void gated_norm_join_kernel(const NormParams 
 }
 
 // How a row is laid over lanes: W waves a row, NC loads of VEC values a lane and operand.  Rows whose width or addresses do
-// not allow aligned loads take the LOOSE form: unaligned ones, and the values of a row's end one by one.
-// One wave a row needs no barrier; four waves bring more of the chip to few rows and leave registers for rows ahead.
-// Forward, bf16 rows of 768, one / four waves: 131 rows 4.4 / 3.9 us, 1024 rows 5.0 / 5.4, 65536 rows 115 / 150.
-// Backward, 16384 rows: 256 wide 25 / 32, 384 33 / 34, 512 38 / 35, 768 49 / 44, 1024 83 / 67; 65536 rows: 256 wide 79 / 117, 512 135 / 150,
-// 640 171 / 171, 768 197 / 195, 1024 273 / 261.
+// not allow aligned loads take the LOOSE form with unaligned ones.  The fewest waves of those built that hold the row in two
+// loads, so that few lanes are left over (backward, 8192 bf16 rows of 2500: 5 waves 64 us, 8 82; of 5000: 10 158, 16 212).
+// One wave a row needs no barrier, and four of them add their sums in LDS; more waves bring more of the chip to few rows.
+// Forward, 768 wide, one / four waves: 131 rows f32 5.6 / 5.3 us, bf16 5.3 / 5.3, 65536 rows 140 / 154 and 114 / 137; 1024 wide
+// 186 / 192 and 154 / 151: one wave up to there.
+// Backward, one / three or four waves: 512 wide 131 rows 8.7 / 7.8, 1024 rows 12.3 / 11.6, 16384 rows f32 35.6 / 44.8; 768 wide 1024 rows
+// 14.6 / 12.2, 8192 rows f32 30.1 / 28.3, bf16 25.5 / 26.5, 65536 rows 214 / 211 and 152 / 162; 600 wide 65536 rows 173 / 181 and 122 / 148.
 struct Shape {
     int W, nc;
 };
 Shape row_shape(int E, bool one_wave) {
-    const int W = one_wave ? 1 : E <= 2048 ? 4 : E <= 4096 ? 8 : 16;
+    int W = one_wave ? 1 : 4;
+    if (!one_wave)
+        for (const int more : {5, 6, 8, 10, 12, 16})
+            if (E > 64 * VEC * 2 * W) W = more;
     return Shape{W, (E + 64 * VEC * W - 1) / (64 * VEC * W)};
 }
-Shape fwd_shape(long M, int E) { return row_shape(E, E <= 1024 && M >= 512); }
-Shape bwd_shape(int E) { return row_shape(E, E <= 512); }
+Shape fwd_shape(int E) { return row_shape(E, E <= 1024); }
+Shape bwd_shape(long M, int E) {
+    const bool one_wave = E <= 512 || (E <= 768 && M >= 8192);
+    return !one_wave && E <= 768 ? Shape{3, 1} : row_shape(E, one_wave);
+}
 
 struct BwdPlan {
     int teams, rows_per_team, teams_per_group, workgroups;
@@ -453,18 +500,15 @@ struct BwdPlan {
 };
 BwdPlan bwd_plan(int M, int E, int G) {
     BwdPlan w{};
-    const int W = bwd_shape(E).W;
+    const int W = bwd_shape(M, E).W;
     const int per_wg = W == 1 ? 4 : 1;
-    // Teams: at most as many as fill the chip once (65536 x 768 bf16, four waves: 1024 teams 195 us, 768 219, 1536 237, 2048 202).
-    // Several waves: every workgroup leaves 4 E sums to be written and joined, 12 us for 1024 of them, and every further row
-    // costs a workgroup 1 us, so rows * 1 us + M / rows * 12 ns is least at the root of M / 85 (1024 x 768 bf16: 1 row 18.9 us,
-    // 2 13.7, 4 12.7, 8 15.9).
-    const int want = W == 1 ? 2048 : 4096 / W;
+    // Teams: as many workgroups as the CUs take alike, one each, or two of three or four waves (16384 x 768 bf16: 512 teams 38.5 us,
+    // 683 40.1, 1024 37.5, 1365 44.1; 16384 x 4096: 256 189, 512 202, 683 213).  Every workgroup leaves 4 E sums to be written and
+    // joined, so it takes a few rows even where the chip is not full (1024 x 768: 1 row 17.7 us, 2 12.9, 4 11.8, 8 13.9).
+    const int want = W == 1 ? 1024 : W <= 4 ? 512 : 256;
+    const int least = M >= 768 ? 4 : M >= 192 ? 2 : 1;
     int rows = (int)(((long)M + want - 1) / want);
-    if (W > 1) {
-        const int even = (int)(sqrt((double)M / 85.0) + 0.5);
-        rows = rows > even ? rows : even;
-    }
+    rows = rows > least ? rows : least;
     const int group = G > 0 ? M / G : 0;
     if (G == 0 || group <= rows) {
         w.rows_per_team = G == 0 ? rows : rows / group * group;
@@ -492,24 +536,33 @@ int check_common(const char *who, int dtype, int gate_dtype, const void *gate, l
 }  // namespace
 
 // the shapes that fwd_shape and bwd_shape name, as W * 10 + NC
-#define TC_GN_COMMON(K, T, TG, LOOSE)                                                           \
-            case 11: TC_GN(K, T, TG, LOOSE, 1, 1); break;                                       \
-            case 12: TC_GN(K, T, TG, LOOSE, 1, 2); break;                                       \
-            case 41: TC_GN(K, T, TG, LOOSE, 4, 1); break;                                       \
-            case 42: TC_GN(K, T, TG, LOOSE, 4, 2); break;                                       \
-            case 82: TC_GN(K, T, TG, LOOSE, 8, 2); break;                                       \
-            default: TC_GN(K, T, TG, LOOSE, 16, 2); break;
+#define TC_GN_COMMON(T, TG, LOOSE)                                                              \
+            case 11: TC_GN(T, TG, LOOSE, 1, 1); break;                                          \
+            case 12: TC_GN(T, TG, LOOSE, 1, 2); break;                                          \
+            case 13: TC_GN(T, TG, LOOSE, 1, 3); break;                                          \
+            case 42: TC_GN(T, TG, LOOSE, 4, 2); break;                                          \
+            case 52: TC_GN(T, TG, LOOSE, 5, 2); break;                                          \
+            case 62: TC_GN(T, TG, LOOSE, 6, 2); break;                                          \
+            case 82: TC_GN(T, TG, LOOSE, 8, 2); break;                                          \
+            case 102: TC_GN(T, TG, LOOSE, 10, 2); break;                                        \
+            case 122: TC_GN(T, TG, LOOSE, 12, 2); break;                                        \
+            default: TC_GN(T, TG, LOOSE, 16, 2); break;
 #define TC_GN_FWD(T, TG, LOOSE)                                                                 \
     do {                                                                                        \
-        switch (sh.W * 10 + sh.nc) {                                                            \
-            case 13: TC_GN(gated_norm_kernel, T, TG, LOOSE, 1, 3); break;                       \
-            case 14: TC_GN(gated_norm_kernel, T, TG, LOOSE, 1, 4); break;                       \
-            TC_GN_COMMON(gated_norm_kernel, T, TG, LOOSE)                                       \
+        if (E < VEC) TC_GN_V(T, TG, false, 1, 1, 1);                                            \
+        else switch (sh.W * 10 + sh.nc) {                                                       \
+            case 14: TC_GN(T, TG, LOOSE, 1, 4); break;                                          \
+            TC_GN_COMMON(T, TG, LOOSE)                                                          \
         }                                                                                       \
     } while (0)
 #define TC_GN_BWD(T, TG, LOOSE)                                                                 \
     do {                                                                                        \
-        switch (sh.W * 10 + sh.nc) { TC_GN_COMMON(gated_norm_bwd_kernel, T, TG, LOOSE) }        \
+        if (E < VEC) TC_GN_V(T, TG, false, 1, 1, 1);                                            \
+        else switch (sh.W * 10 + sh.nc) {                                                       \
+            case 31: TC_GN(T, TG, LOOSE, 3, 1); break;                                          \
+            case 41: TC_GN(T, TG, LOOSE, 4, 1); break;                                          \
+            TC_GN_COMMON(T, TG, LOOSE)                                                          \
+        }                                                                                       \
     } while (0)
 #define TC_GN_L(K, T, TG)                                                                       \
     do {                                                                                        \
@@ -550,17 +603,20 @@ extern "C" int tc_gated_residual_norm_fwd(int dtype, const void *y, long ldy, co
     const bool loose = !(tc_rows_aligned(y, ldy, esz, VEC) && tc_rows_aligned(x, ldx, 4, VEC) && tc_rows_aligned(gate, E, g_esz, VEC) &&
                tc_rows_aligned(h, E, esz, VEC) && tc_rows_aligned(x_out, E, 4, VEC) && tc_rows_aligned(post_gamma, 0, 4, VEC) &&
                tc_rows_aligned(post_beta, 0, 4, VEC) && tc_rows_aligned(pre_gamma, 0, 4, VEC) && tc_rows_aligned(pre_beta, 0, 4, VEC));
-    const Shape sh = fwd_shape(M, E);
+    const Shape sh = fwd_shape(E);
     const int per_wg = sh.W == 1 ? 4 : 1;
     long blocks = (M + per_wg - 1) / per_wg;
     // rows are walked with the grid's stride: a launch holds fewer than 2^32 threads, and teams that ask ahead fill the chip once
-    const long most = sh.W == 16 ? 512 : 1L << 21;
+    const long most = sh.W > 8 ? 256 : sh.W > 4 ? 512 : 1L << 21;
     if (blocks > most) blocks = most;
     hipStream_t s = static_cast<hipStream_t>(stream);
     TcProfScope prof(TC_PROF_LAYERNORM, s, (double)M * E * (2 * esz + 8));
-#define TC_GN(K, T, TG, L, WW, N) TC_LAUNCH((K<T, TG, L, WW, N>), dim3((unsigned)blocks), dim3(WW == 1 ? 256 : 64 * WW), 0, s, p)
+#define TC_GN_V(T, TG, L, WW, N, V) \
+    TC_LAUNCH((gated_norm_kernel<T, TG, L, WW, N, V>), dim3((unsigned)blocks), dim3(WW == 1 ? 256 : 64 * WW), 0, s, p)
+#define TC_GN(T, TG, L, WW, N) TC_GN_V(T, TG, L, WW, N, VEC)
     TC_GN_T(TC_GN_FWD);
 #undef TC_GN
+#undef TC_GN_V
     TC_CHECK_LAUNCH("tc_gated_residual_norm_fwd");
     return TC_OK;
 }
@@ -611,7 +667,7 @@ extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh,
                (!dh || tc_rows_aligned(dh, ld_dh, esz, VEC)) && (!dx_out || tc_rows_aligned(dx_out, ld_dxo, 4, VEC)) &&
                tc_rows_aligned(dy, E, esz, VEC) && tc_rows_aligned(dx, E, 4, VEC) && tc_rows_aligned(d_gate, E, 4, VEC) &&
                tc_rows_aligned(post_gamma, 0, 4, VEC) && tc_rows_aligned(post_beta, 0, 4, VEC) && tc_rows_aligned(pre_gamma, 0, 4, VEC));
-    const Shape sh = bwd_shape(E);
+    const Shape sh = bwd_shape(M, E);
     const BwdPlan w = bwd_plan((int)M, E, G);
     NormParams p{};
     p.y = y; p.x = x_out; p.gate = gate; p.dh = dh; p.dx_out = dx_out;
@@ -628,10 +684,13 @@ extern "C" int tc_gated_residual_norm_bwd(int dtype, const void *dh, long ld_dh,
     p.teams = w.teams; p.rows_per_team = w.rows_per_team; p.teams_per_group = w.teams_per_group;
     hipStream_t s = static_cast<hipStream_t>(stream);
     TcProfScope prof(TC_PROF_LAYERNORM, s, (double)M * E * (3 * esz + 12));
-#define TC_GN(K, T, TG, L, WW, N)                                                                                         \
-    TC_LAUNCH((K<T, TG, L, WW, N>), dim3((unsigned)w.workgroups), dim3(WW == 1 ? 256 : 64 * WW), WW == 1 ? 16 * (size_t)E : 0, s, p)
+#define TC_GN_V(T, TG, L, WW, N, V)                                                                                        \
+    TC_LAUNCH((gated_norm_bwd_kernel<T, TG, L, WW, N, V>), dim3((unsigned)w.workgroups), dim3(WW == 1 ? 256 : 64 * WW),     \
+              WW == 1 ? 16 * (size_t)E : 0, s, p)
+#define TC_GN(T, TG, L, WW, N) TC_GN_V(T, TG, L, WW, N, VEC)
     TC_GN_T(TC_GN_BWD);
 #undef TC_GN
+#undef TC_GN_V
     const int groups = w.teams_per_group > 0 ? G : 0;
     const int tall = 4 + groups < 1024 ? 4 + groups : 1024;
     TC_LAUNCH(gated_norm_join_kernel, dim3((E + 63) / 64, tall), dim3(1024), 0, s, p, w.workgroups, groups);
