@@ -394,7 +394,7 @@ def test_results_in_place_of_the_residual_stream(E, second):
 @pytest.mark.parametrize("E", [1, 2, 3, 5, 257, 513, 769, 1025, 2049, 4097, 8191])
 @pytest.mark.parametrize("G", [0, 1, 5, 40])
 def test_a_row_end_behind_the_last_whole_piece(E, G):
-    """The columns that two lanes hold count once in every sum; the rows next to the result are left as they were."""
+    """The columns that two lanes hold count once in every sum."""
     c = _case(40, E, torch.float32, G, False)
     g = _on_gpu(c)
     x_out, h, stats = ops.gated_residual_norm(g["y"], g["x"], g["post_gamma"], g["post_beta"], g["gate"], g["pre_gamma"], g["pre_beta"])
@@ -407,3 +407,40 @@ def test_a_row_end_behind_the_last_whole_piece(E, G):
         assert a is None and b is None or torch.equal(a + 1.0, b)
     # a gradient of beta is a plain sum over the rows of dh: 40 values of size up to 4, f32
     assert float((got[6].double().cpu() - c["dh"].double().sum(0)).abs().max()) <= 40 * 4 * 40 * 2.0 ** -24
+
+
+@gpu
+@pytest.mark.parametrize("E", [1, 3, 5, 255, 514, 769, 1025, 2050, 4099, 8191])
+@pytest.mark.parametrize("first", [0, 1])
+def test_what_lies_around_the_results_is_left_as_it_was(E, first):
+    """Dense results at any address, guards of 64 values on both sides."""
+    M, G, lib = 30, 5, _lib.load()
+    c = _on_gpu(_case(M, E, torch.bfloat16, G, False))
+    guards = []
+
+    def result(*shape, dtype=torch.float32):
+        size = torch.Size(shape).numel()
+        buf = torch.full((size + 129,), 7.0, dtype=dtype, device=DEV)
+        guards.append((buf, 64 + first, 64 + first + size))
+        return buf[64 + first:64 + first + size].view(shape)
+
+    P = lambda t: t.data_ptr()
+    stream = torch.cuda.current_stream().cuda_stream
+    x_out, h, stats = result(M, E), result(M, E, dtype=torch.bfloat16), torch.empty(M, 4, device=DEV)
+    assert lib.tc_gated_residual_norm_fwd(1, P(c["y"]), E, P(c["x"]), E, P(c["post_gamma"]), P(c["post_beta"]), 0, P(c["gate"]), G, 1.0,
+                                          P(c["pre_gamma"]), P(c["pre_beta"]), P(x_out), P(h), P(stats), M, E, 0, 1e-5, 1e-5, stream) == 0
+    want = ops.gated_residual_norm(c["y"], c["x"], c["post_gamma"], c["post_beta"], c["gate"], c["pre_gamma"], c["pre_beta"])
+    assert torch.equal(x_out, want[0]) and torch.equal(h, want[1]) and torch.equal(stats, want[2])
+    dy, dx, d_gate, vectors = result(M, E, dtype=torch.bfloat16), result(M, E), result(G, E), [result(E) for _ in range(4)]
+    need = lib.tc_gated_residual_norm_bwd_workspace_bytes(M, E, G)
+    ws = torch.full((need + 64,), 77, dtype=torch.uint8, device=DEV)
+    assert lib.tc_gated_residual_norm_bwd(1, P(c["dh"]), E, P(c["dx_out"]), E, P(c["y"]), E, P(x_out), E, P(stats), P(c["post_gamma"]),
+                                          P(c["post_beta"]), 0, P(c["gate"]), G, 1.0, P(c["pre_gamma"]), P(dy), P(dx), P(vectors[0]),
+                                          P(vectors[1]), P(d_gate), P(vectors[2]), P(vectors[3]), 0, M, E, 0, P(ws), need, stream) == 0
+    back = ops.gated_residual_norm_bwd(c["dh"], c["dx_out"], c["y"], want[0], stats, c["post_gamma"], c["post_beta"], c["gate"],
+                                       c["pre_gamma"], c["pre_beta"])
+    for a, b in zip([dy, dx, vectors[0], vectors[1], d_gate, vectors[2], vectors[3]], back):
+        assert torch.equal(a, b)
+    assert bool((ws[need:] == 77).all())
+    for buf, begin, end in guards:
+        assert bool((buf[:begin] == 7.0).all()) and bool((buf[end:] == 7.0).all())
