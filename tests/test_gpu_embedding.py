@@ -215,3 +215,35 @@ def test_rows_without_a_position_are_zeros_for_any_scale(rows):
     want = torch.zeros(6, 8, device=DEV)
     want[3] = float("inf")
     assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("pad", [None, 1])
+def test_the_smallest_ids_are_flagged_and_left_out(pad):
+    """The ends of the id types (what a bad conversion from a float leaves) are out of range like any other, with and without
+    a padding id."""
+    table = torch.ones(5, 8, device=DEV)
+    for idt in (torch.int32, torch.int64):
+        ends = torch.iinfo(idt)
+        for odd in (ends.min, ends.min + 1, -2, -1, 5, ends.max):
+            ids = torch.tensor([2, odd, 3], dtype=idt, device=DEV)
+            bad = torch.zeros(1, dtype=torch.int32, device=DEV)
+            out = ops.embedding(ids, table, 2.0, pad_idx=pad, bad=bad).cpu()
+            assert int(bad) == 1, (idt, odd)
+            assert torch.equal(out, torch.tensor([2.0, 0.0, 2.0])[:, None].expand(3, 8))
+            for rows in (3, 600):                                 # without and with a sort
+                dy = torch.ones(rows, 8, device=DEV)
+                got = ops.embedding_bwd(ids.repeat(rows // 3), dy, 5, 1.0, pad_idx=pad).cpu()
+                assert torch.equal(got[:, 0], torch.tensor([0.0, 0.0, rows / 3, rows / 3, 0.0])), (idt, odd, rows)
+
+
+@gpu
+def test_any_negative_padding_id_stands_for_none():
+    """tc_embedding_fwd: pad_idx < 0 is no padding id, so an id of that very value is out of range."""
+    lib, table = _lib.load(), torch.ones(5, 8, device=DEV)
+    for pad in (-1, -7, -2 ** 63):
+        ids = torch.tensor([2, pad], device=DEV)
+        bad, out = torch.zeros(1, dtype=torch.int32, device=DEV), torch.full((2, 8), 3.0, device=DEV)
+        assert lib.tc_embedding_fwd(0, 0, 8, ids.data_ptr(), table.data_ptr(), out.data_ptr(), 2, 8, 5, 1.0, pad, bad.data_ptr(),
+                                    torch.cuda.current_stream().cuda_stream) == 0
+        assert int(bad) == 1 and torch.equal(out.cpu(), torch.tensor([1.0, 0.0])[:, None].expand(2, 8))

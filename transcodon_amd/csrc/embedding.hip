@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void embedding_kernel(const TID *__restrict__ 
     const long step = (long)gridDim.x * 256 >> lanes_log2;
     for (long row = ((long)blockIdx.x * 256 + threadIdx.x) >> lanes_log2; row < M; row += step) {
         const long tok = (long)tokens[row];
-        const bool pad = tok == pad_idx;
+        const bool pad = pad_idx >= 0 && tok == pad_idx;      // no id below 0 is padding, whatever pad_idx is
         const bool out_of_range = !pad && (tok < 0 || tok >= vocab);
         if (out_of_range && bad && sub == 0) *bad = 1;
         TO *dst = out + row * E;
@@ -596,7 +596,6 @@ extern "C" int tc_embedding_fwd(int table_dtype, int out_dtype, int id_bytes, co
     const int t_esz = table_dtype == TC_BF16 ? 2 : 4, o_esz = out_dtype == TC_BF16 ? 2 : 4;
     TC_REQUIRE((uintptr_t)table % t_esz == 0 && (uintptr_t)out % o_esz == 0 && (uintptr_t)tokens % id_bytes == 0,
                "tc_embedding_fwd: misaligned operand");
-    if (pad_idx < 0) pad_idx = INT64_MIN;          // no padding id
     // 16-byte stores, 4 f32 or 8 bf16 values; rows that start anywhere or end inside a piece take the loose form
     const int wide = out_dtype == TC_BF16 ? 8 : 4;
     const bool loose = !(tc_rows_aligned(table, E, t_esz, wide) && tc_rows_aligned(out, E, o_esz, wide));
@@ -648,7 +647,6 @@ extern "C" int tc_embedding_bwd(int dy_dtype, int id_bytes, const void *tokens, 
         tc_set_error("tc_embedding_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, w.total);
         return TC_ENOSPC;
     }
-    if (pad_idx < 0) pad_idx = INT64_MIN;
     char *ws = static_cast<char *>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool loose = !(tc_rows_aligned(dy, ld_dy, esz, VEC) && tc_rows_aligned(d_table, E, 4, VEC));
