@@ -307,3 +307,33 @@ def test_weight_gradient_takes_scales_of_any_byte(rows):
     # a product with a value below the smallest normal number may count as zero on the matrix cores
     assert bool(((got[:, :255 * 32] - want[:, :255 * 32]).abs() <= 2.0 ** -126).all())
     assert torch.equal(got[:, 2 * 32:255 * 32], want[:, 2 * 32:255 * 32])
+
+
+def test_weight_gradient_workspace_is_bounded_without_a_gpu():
+    """At most 128 MiB or a quarter of the operands' bytes, whatever the shape; rows behind the last whole stage take no part of
+    the sum of their own."""
+    need = _lib.load().tc_gemm_tn_act8_workspace_bytes
+    gen = torch.Generator().manual_seed(3)
+    size = lambda lo, hi: int(2.0 ** (lo + (hi - lo) * float(torch.rand(1, generator=gen))))
+    shapes = [(231953, 13736, 12176), (100000, 8192, 8192), (50000, 20000, 20000), (65536, 2304, 768), (2 ** 31 - 100, 8, 16)]
+    shapes += [(size(0, 24), size(0, 13) * 8, size(0, 12) * 16) for _ in range(3000)]
+    for M, N, K in shapes:
+        for rows in (M, M // 64 * 64 or M):
+            got = need(rows, N, N, K)
+            assert 0 < got <= max(128 * 2 ** 20, rows * (2 * N + K) // 4), (rows, N, K, got)
+            assert got == 16 or got % (4 * N * K) == 0
+    assert need(3400, 4096, 4096, 4096) == need(3392, 4096, 4096, 4096) == 16
+
+
+@gpu
+@pytest.mark.parametrize("M", [3393, 3400, 3455, 8193, 8255])
+@pytest.mark.parametrize("N,K", [(4096, 4096), (2304, 784)])
+def test_weight_gradient_counts_the_last_rows_once(M, N, K):
+    """Whole stages are ones in dy, the rows behind them twos: sums of small whole numbers, exact in any order."""
+    dy = torch.ones(M, N, dtype=torch.bfloat16, device=DEV)
+    dy[M // 64 * 64:] = 2.0
+    codes, scales = ops.act8_pack(torch.ones(M, K, device=DEV))
+    want = float(M + M % 64)
+    assert bool((ops.gemm_tn_act8(dy, codes, scales) == want).all())
+    out = torch.full((N, K), 5.0, device=DEV)
+    assert bool((ops.gemm_tn_act8(dy, codes, scales, out=out) == want + 5.0).all())

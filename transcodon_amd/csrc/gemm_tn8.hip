@@ -449,9 +449,10 @@ bool tn8_dims_ok(long M, int N, int K) {
 
 struct Tn8Plan {
     bool big;                // 256 x 256 tiles over the whole stages, the rows behind them by the small kernel
-    int splits, slabs;
+    int splits;              // row splits, and parts of the sum
 };
 constexpr int kManySlabs = 16;
+constexpr long kPartBytes = 128L << 20;      // what the parts of a sum may always take; else a quarter of the operands' bytes
 // Which kernel and how many row splits: the least estimated time over both kernels and up to 256 splits, in nanoseconds.
 // A stage takes a large tile 1.9 us on a full chip (220 us at 65536 x 2304 x 768: 114 stages), a small one 1 us while
 // there is one workgroup per CU and 0.6 us more for each further one; a part of the sum costs its slab written and read at
@@ -461,25 +462,27 @@ Tn8Plan tn8_plan(long M, long ld_dy, int N, int K) {
     long least = -1;
     const long nk = (M + KT - 1) / KT, whole = M / KT;
     const long large = (long)((N + 255) / 256) * ((K + 255) / 256), small = (long)((N + 127) / 128) * ((K + 127) / 128);
+    const long quarter = M * (2L * N + K) / 4, most = quarter > kPartBytes ? quarter : kPartBytes;
     auto parts = [&](long slabs) { return slabs > 1 ? 4000 + slabs * N * K * 8 / 6500 : 0; };
     for (long s = 1; s <= 256; s += s < 16 ? 1 : s < 64 ? 4 : 16) {
+        if (s > 1 && s * N * K * 4 > most) break;
         if (s >= kManySlabs && (long)N * K > (1L << 29)) break;      // tn8_sum_kernel's launch holds fewer than 2^32 threads
         if (s <= nk) {
             const long wgs = small * s;
             const long ns = 2000 + (nk + s - 1) / s * (400 + 600 * (wgs > 256 ? wgs : 256) / 256) + parts(s);
             if (least < 0 || ns < least) {
                 least = ns;
-                best = Tn8Plan{false, (int)s, (int)s};
+                best = Tn8Plan{false, (int)s};
             }
         }
         // offsets inside a split, with the stages loaded ahead, are 32 bits
         const long rows = (whole / s + 4) * KT;
         if (whole >= 2 * s && rows * ld_dy * 2 < (1L << 32) && rows * K < (1L << 32)) {
-            const int rest = M % KT != 0;          // the rows behind the whole stages: one more part and launch
-            const long ns = 3000 + (whole + s - 1) / s * 1900 * ((large * s + 255) / 256) + 5000 * rest + parts(s + rest);
+            const int rest = M % KT != 0;          // the rows behind the whole stages: one more launch
+            const long ns = 3000 + (whole + s - 1) / s * 1900 * ((large * s + 255) / 256) + 5000 * rest + parts(s);
             if (ns < least) {
                 least = ns;
-                best = Tn8Plan{true, (int)s, (int)s + rest};
+                best = Tn8Plan{true, (int)s};
             }
         }
     }
@@ -490,8 +493,8 @@ Tn8Plan tn8_plan(long M, long ld_dy, int N, int K) {
 
 extern "C" size_t tc_gemm_tn_act8_workspace_bytes(long M, long ld_dy, int N, int K) {
     if (!tn8_dims_ok(M, N, K) || ld_dy < N) return 0;
-    const int slabs = tn8_plan(M, ld_dy, N, K).slabs;
-    return slabs > 1 ? (size_t)slabs * N * K * sizeof(float) : 16;
+    const int parts = tn8_plan(M, ld_dy, N, K).splits;
+    return parts > 1 ? (size_t)parts * N * K * sizeof(float) : 16;
 }
 
 extern "C" int tc_gemm_tn_act8(const void *dy, long ld_dy, const void *codes, const void *scales, float *dW, long M, int N, int K,
@@ -515,9 +518,9 @@ extern "C" int tc_gemm_tn_act8(const void *dy, long ld_dy, const void *codes, co
     p.M = (int)M; p.N = N; p.K = K;
     p.groups = (K + kAct8Group - 1) / kAct8Group;
     p.splits = w.splits;
-    p.out = w.slabs > 1 ? static_cast<float *>(workspace) : dW;
+    p.out = w.splits > 1 ? static_cast<float *>(workspace) : dW;
     p.slab_elems = (long)N * K;
-    p.accumulate = w.slabs > 1 ? 0 : accumulate;
+    p.accumulate = w.splits > 1 ? 0 : accumulate;
     hipStream_t s = static_cast<hipStream_t>(stream);
     static_assert(LDS_BYTES <= 64 * 1024, "no attribute needed");
     const dim3 small_grid((unsigned)(((N + 127) / 128) * ((K + 127) / 128)), (unsigned)w.splits);
@@ -539,17 +542,16 @@ extern "C" int tc_gemm_tn_act8(const void *dy, long ld_dy, const void *codes, co
         p.nk = (int)(M / KT);
         p.tiles_k = (K + 255) / 256;
         TC_LAUNCH(gemm_tn8_256_kernel, dim3((unsigned)(((N + 255) / 256) * p.tiles_k), (unsigned)w.splits), dim3(512), big::LDS_BYTES, s, p);
-        if (M % KT != 0) {                         // the last rows: a part of their own
+        if (M % KT != 0) {                         // the last rows: added to the first part
             const long done = M / KT * KT;
             Tn8Params t = p;
-            t.accumulate = 0;
+            t.accumulate = 1;
             t.dy += done * p.ld_bytes;
             t.codes += done * K;
             t.scales += done * p.groups;
             t.M = (int)(M - done);
             t.nk = t.splits = 1;
             t.tiles_k = (K + 127) / 128;
-            t.out += w.splits * p.slab_elems;
             TC_LAUNCH(gemm_tn8_kernel, dim3(small_grid.x, 1), dim3(256), LDS_BYTES, s, t);
         }
     } else {
@@ -557,10 +559,10 @@ extern "C" int tc_gemm_tn_act8(const void *dy, long ld_dy, const void *codes, co
         p.tiles_k = (K + 127) / 128;
         TC_LAUNCH(gemm_tn8_kernel, small_grid, dim3(256), LDS_BYTES, s, p);
     }
-    if (w.slabs > kManySlabs) {
+    if (w.splits > kManySlabs) {
         const long n4 = (long)N * K / 4;
-        TC_LAUNCH(tn8_sum_kernel, dim3((unsigned)((n4 + 63) / 64)), dim3(1024), 0, s, p.out, dW, w.slabs, n4, accumulate);
+        TC_LAUNCH(tn8_sum_kernel, dim3((unsigned)((n4 + 63) / 64)), dim3(1024), 0, s, p.out, dW, w.splits, n4, accumulate);
     }
     TC_CHECK_LAUNCH("tc_gemm_tn_act8");
-    return w.slabs > 1 && w.slabs <= kManySlabs ? tc_reduce_slabs(p.out, dW, w.slabs, (long)N * K, accumulate, stream) : TC_OK;
+    return w.splits > 1 && w.splits <= kManySlabs ? tc_reduce_slabs(p.out, dW, w.splits, (long)N * K, accumulate, stream) : TC_OK;
 }
