@@ -613,9 +613,11 @@ typedef struct tc_encoder_grads {
 /*
  * Bytes of workspace for tc_encoder_forward_train + tc_encoder_backward on a [B,T] batch.  With desc->act8 the two LayerNorm
  * outputs and the fc1 pre-activation of each layer are kept as e4m3 codes with one power of two per 32 values and gelu's output
- * not at all: 22 E + 4 H bytes a token and layer instead of 36 E + 4 H (F = 4 E).  The forward pass computes the same values either way; the
- * gradients see the rounded ones (weight gradients of q/k/v, fc1 and fc2, and gelu').  desc->act8 must be the same in
- * all three calls.
+ * not at all: 22 E + 4 H bytes a token and layer instead of 36 E + 4 H (F = 4 E).  The forward pass computes the same values either way.
+ * In the backward pass the weight gradients of q/k/v, fc1 and fc2 and gelu' are taken at the 8-bit values; the gradient of gelu's output
+ * is rounded to bf16 before gelu' multiplies it (without act8 that product is taken in f32), and fc1's bias gradient is the
+ * sum of the bf16 gradients of fc1's output (without act8: of the f32 ones).  So every gradient changes but those of the heads, the
+ * final LayerNorm and the last layer's fc2 bias.  desc->act8 must be the same in all three calls.
  */
 size_t tc_train_workspace_bytes(const tc_encoder_desc *desc, int B, int T);
 

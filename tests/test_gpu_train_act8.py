@@ -1,6 +1,7 @@
 """Training with 8-bit activation checkpoints (model.act8_checkpoints): the same forward pass, less memory, gradients near those of the
 bf16 checkpoints."""
 import ctypes as C
+import dataclasses
 
 import pytest
 import torch
@@ -123,3 +124,40 @@ def test_workspace_is_smaller():
     assert abs(saved - tokens * (36 - 22.1875) * 768 - tokens * 256) < 2 ** 20 * 64       # the rows' 128-byte gaps; split-sum buffers
     d.dtype = _lib.TC_F32
     assert lib.tc_train_workspace_bytes(C.byref(d), 64, 1024) == 0
+
+
+ABOVE = ("lm_head.", "structure_linear.", "emb_layer_norm_after.")            # no 8-bit value on the way to these
+
+
+def _gradients_change_where_they_should(cfg, B, T):
+    m = _model(cfg)
+    batch = _batch(cfg, B, T)
+    logits16, _, want = _step(m, batch, False)
+    logits8, _, got = _step(m, batch, True)
+    assert torch.equal(logits8, logits16)
+    assert set(got) == set(want)
+    off = {k: float((got[k] - w).norm() / (w.norm() + 1e-12)) for k, w in want.items()}
+    top = f"layers.{cfg.num_layers - 1}.fc2.bias"
+    assert top in off
+    for k, d in off.items():
+        assert bool(torch.isfinite(got[k]).all()), k
+        if k.startswith(ABOVE) or k == top:
+            assert d <= 1e-4, (k, d)                              # additions by atomics, in any order
+        else:
+            assert d <= 0.12, (k, d)                              # as derived above for two layers
+        if k.startswith("layers.") and k.endswith(("q_proj.weight", "k_proj.weight", "v_proj.weight", "fc1.weight", "fc2.weight")):
+            assert d > 2e-4, (k, d)                               # 8-bit values did enter: more than the atomics explain
+
+
+@gpu
+@pytest.mark.parametrize("B,T", [(3, 40), (5, 64), (2, 131)])
+def test_gradients_change_where_the_8_bit_values_enter(B, T):
+    _gradients_change_where_they_should(O.TINY, B, T)
+
+
+@gpu
+@pytest.mark.parametrize("B,T", [(7, 1171), (5, 500)])
+def test_one_layer_of_full_width(B, T):
+    """Enough rows for the weight gradients' 256 x 256 tiles in several parts, with rows behind the last whole stage (8197 = 128 * 64 + 5),
+    beside the buffers that they share with the rest of the step; 2500 rows take the small tiles."""
+    _gradients_change_where_they_should(dataclasses.replace(O.FULL, num_layers=1), B, T)

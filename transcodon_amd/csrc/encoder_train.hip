@@ -187,7 +187,8 @@ int linear_wgrad(const tc_encoder_desc *d, TrainWs &w, int in_dt, const void *dy
     return TC_OK;
 }
 
-// The same with X kept in 8 bits (bf16 dY): codes and scales straight into the product.
+// The same with X kept in 8 bits: codes and scales straight into the product.  dY is bf16, its column sums are those of the
+// rounded values (the f32 ones are never in memory).
 int linear_wgrad8(TrainWs &w, const void *dy, int ld_dy, const void *codes, const void *scales, int M, int n_out, int n_in, float *dW,
                   float *dbias, void *stream) {
     TC_TRY(tc_colsum(TC_BF16, dy, ld_dy, nullptr, 0, dbias, M, n_out, stream));
@@ -394,6 +395,8 @@ extern "C" int tc_encoder_backward_notify(const tc_encoder_desc *d, const tc_enc
         int ld_du = w.ld_f;
         if (d->act8) {
             // gelu's output again and its gradient, from the 8-bit input in one pass; both are dense in the transposes' buffers
+            // The product's result is rounded to bf16 before gelu' (2^-8 of it at most, as a bf16 linear layer returns it), half the
+            // bytes of an f32 one to write and read again; gelu' itself is off by up to 2^-5 through the 8-bit input.
             TC_TRY(tc_gemm(dt, TC_EPI_BIAS, w.dyb, E, wt_of(d, w, l, WT_FC2), nullptr, nullptr, w.wide, w.ld_f, M, F, E, 0.f, nullptr,
                            nullptr, 0, 0, stream));
             TC_TRY(tc_dgelu_act8(dt, w.wide, w.ld_f, sv.u_c, sv.u_s, w.tr_a, w.tr_b, M, F, stream));
