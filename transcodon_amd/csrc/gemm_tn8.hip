@@ -2,7 +2,7 @@
 //   dW[N,K] = sum_m dY[m,N] * X[m,K]     dY bf16 [M, ld], X as e4m3 codes [M,K] and one power of two per row and 32 columns
 //
 // The reduction runs over the rows of both operands, and the scale of X changes with the row: it cannot be taken out of
-// the sum.  A code times its power of two is a bf16 number exactly (4 significand bits), so the codes are expanded to
+// the sum.  A code times its power of two is a bf16 number exactly (4 significand bits; from 2^-133 up), so the codes are expanded to
 // bf16 on their way into LDS and the product runs on the bf16 matrix cores with f32 accumulators: no rounding but that
 // of the f32 sums.  dY goes to LDS by direct loads; fragments of both are taken with the transposing LDS read.
 // Two kernels: 128 x 128 output tiles for small products and the last rows, 256 x 256 tiles with two wave groups in
