@@ -4,6 +4,9 @@ Tolerances follow the arithmetic.  C = 2^-24 is half a step of f32.  A row sum i
 and 8 across waves, so with the few operations around it every f32 intermediate is within K C of the sum of the magnitudes that
 enter it, K = 64; errors of inputs are carried on through the derivative.  A column sum of n rows is within n C of the sum of
 its terms' magnitudes.  Results rounded to bf16 are off by another 2^-8 of the value."""
+import os
+import re
+
 import pytest
 import torch
 
@@ -444,3 +447,104 @@ def test_what_lies_around_the_results_is_left_as_it_was(E, first):
     assert bool((ws[need:] == 77).all())
     for buf, begin, end in guards:
         assert bool((buf[:begin] == 7.0).all()) and bool((buf[end:] == 7.0).all())
+
+
+# ---- every layout of rows over waves ----------------------------------------------------------------
+# The kernels exist for (waves a row, loads a lane), each for aligned rows and for any rows.  Widths and row counts below reach all of
+# them in both directions; the tolerances are those above (a row sum of at most 16 waves: 8 additions in a lane, 6 across a
+# wave, 16 across waves, or of one wave 16 and 6: below K).
+def _shape(M, E, backward):
+    """(waves, loads of four columns a lane) as the dispatch takes them."""
+    if backward and 512 < E <= 768 and M < 8192:
+        return 3, 1
+    W = 1 if E <= ((768 if M >= 8192 else 512) if backward else 1024) else 4
+    if W > 1:
+        for more in (5, 6, 8, 10, 12, 16):
+            if E > 512 * W:
+                W = more
+    return W, -(-E // (256 * W))
+
+
+FEW_ROWS = [(5, E) for E in (96, 255, 260, 511, 600, 767, 1000, 1023, 1500, 1501, 2304, 2305, 2820, 3001, 3500, 3501, 5000, 5001, 6000,
+                             6143, 7000, 8191)]
+MANY_ROWS = [(8192, 768), (8195, 766), (8200, 600)]
+
+
+def test_every_layout_is_tested_without_a_gpu():
+    source = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "gated_norm.hip")).read()
+    common, fwd, bwd = (source[source.index(f"#define {n}("):].split("\n\n")[0].split("#define")[1] for n in
+                        ("TC_GN_COMMON", "TC_GN_FWD", "TC_GN_BWD"))
+    built = lambda text: {(int(w), int(n)) for w, n in re.findall(r"TC_GN\(T, TG, LOOSE, (\d+), (\d+)\)", text)}
+    for backward, text in ((False, fwd), (True, bwd)):
+        there = built(common) | built(text)
+        reached = {_shape(M, E, backward) for M in (1, 700, 8191, 8192) for E in range(4, 8193)}
+        assert reached == there                                   # nothing is built that no call takes, nothing falls to the default
+        for loose in (False, True):
+            tested = {_shape(M, E, backward) for M, E in FEW_ROWS + MANY_ROWS if (E % 4 != 0) == loose}
+            assert tested == there, (backward, loose, there - tested)
+
+
+def _both_directions(M, E, dt, G, rms, gate_dt):
+    res = 0.875
+    c = _case(M, E, dt, G, rms, gate_dt=gate_dt)
+    want_x, ex, want_h, eh = _forward(c, rms, res)
+    g = _on_gpu(c)
+    x_out, h, _ = ops.gated_residual_norm(g["y"], g["x"], g["post_gamma"], g["post_beta"], g["gate"], g["pre_gamma"], g["pre_beta"],
+                                          res_scale=res, rms=rms)
+    assert bool(((x_out.cpu().double() - want_x).abs() <= ex).all())
+    assert bool(((h.cpu().double() - want_h).abs() <= eh).all())
+    x_out = want_x.float()
+    args = (g["dh"], g["dx_out"], g["y"], x_out.to(DEV), _stats64(c, x_out, rms).to(DEV), g["post_gamma"], g["post_beta"], g["gate"],
+            g["pre_gamma"], g["pre_beta"])
+    got = ops.gated_residual_norm_bwd(*args, res_scale=res, rms=rms)
+    _check_backward(c, got, x_out, rms, res)
+    again = ops.gated_residual_norm_bwd(*args, res_scale=res, rms=rms)
+    assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(got, again))
+
+
+@gpu
+@pytest.mark.parametrize("M,E", FEW_ROWS)
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rms", [False, True])
+def test_every_width_class(M, E, dt, rms):
+    for G, gate_dt in ((0, torch.float32), (1, dt), (M, torch.float32), (M, dt)):
+        _both_directions(M, E, dt, G, rms, gate_dt)
+
+
+@gpu
+@pytest.mark.parametrize("M,E,G,rms", [(8192, 768, 0, False), (8192, 768, 64, False), (8192, 768, 8192, True), (8195, 766, 1, False),
+                                       (8195, 766, 5, True), (8195, 766, 8195, False), (8200, 600, 0, True), (8200, 600, 8, False),
+                                       (8200, 600, 4100, False)])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_many_rows_of_one_wave_each(M, E, G, rms, dt):
+    _both_directions(M, E, dt, G, rms, dt if G == M else torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("M,E", [(700, E) for _, E in FEW_ROWS if E > 1024] + MANY_ROWS + [(8192, 511)])
+@pytest.mark.parametrize("second", [True, False])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_results_in_place_in_every_layout(M, E, second, dt):
+    """x_out may be x, and dx may be dx_out."""
+    G, lib = 5 if M % 5 == 0 else 64, _lib.load()
+    c = _on_gpu(_case(M, E, dt, G, False))
+    pre = (c["pre_gamma"], c["pre_beta"]) if second else (None, None)
+    dh = c["dh"] if second else None
+    P = lambda t: None if t is None else t.data_ptr()
+    code, stream = int(dt == torch.bfloat16), torch.cuda.current_stream().cuda_stream
+    x_out, h, stats = ops.gated_residual_norm(c["y"], c["x"], c["post_gamma"], c["post_beta"], c["gate"], *pre, res_scale=0.5)
+    want = ops.gated_residual_norm_bwd(dh, c["dx_out"], c["y"], x_out, stats, c["post_gamma"], c["post_beta"], c["gate"], *pre,
+                                       res_scale=0.5)
+    need = lib.tc_gated_residual_norm_bwd_workspace_bytes(M, E, G)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    x, d, h2, stats2, dy = c["x"].clone(), c["dx_out"].clone(), torch.empty_like(c["y"]), torch.empty_like(stats), torch.empty_like(c["y"])
+    assert lib.tc_gated_residual_norm_fwd(code, P(c["y"]), E, P(x), E, P(c["post_gamma"]), P(c["post_beta"]), 0, P(c["gate"]), G, 0.5, P(pre[0]),
+                                          P(pre[1]), P(x), P(h2) if second else None, P(stats2), M, E, 0, 1e-5, 1e-5, stream) == 0
+    assert torch.equal(x, x_out) and torch.equal(stats2, stats) and (not second or torch.equal(h2, h))
+    grads = [torch.empty_like(t) for t in want[2:] if t is not None]
+    g = grads + [None] * (5 - len(grads))
+    assert lib.tc_gated_residual_norm_bwd(code, P(dh), E, P(d), E, P(c["y"]), E, P(x_out), E, P(stats), P(c["post_gamma"]), P(c["post_beta"]), 0,
+                                          P(c["gate"]), G, 0.5, P(pre[0]), P(dy), P(d), P(g[0]), P(g[1]), P(g[2]), P(g[3]), P(g[4]), 0, M, E, 0,
+                                          P(ws), need, stream) == 0
+    for a, b in zip([dy, d, *grads], [t for t in want if t is not None]):
+        assert torch.equal(a, b)
