@@ -166,20 +166,25 @@ __global__ __launch_bounds__(256) void gemm_tn8_kernel(const Tn8Params p) {
 
     float *out = p.out + (long)blockIdx.y * p.slab_elems;
     const int jl = lane & 31;
+    auto row_of = [&](int a, int r) { return i0 + wi * 64 + a * 32 + (r & 3) + 8 * (r >> 2) + 4 * h2; };
+    auto col_of = [&](int b) { return j0 + wj * 64 + b * 32 + jl; };
+    // What is added to is loaded before the first store, all of it under way together (one after the other: 8197 x 2304 x 784 80
+    // instead of 65 us); places past the ends read the last one.
+    if (p.accumulate) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[a][b][r] += out[(long)min(row_of(a, r), p.N - 1) * p.K + min(col_of(b), p.K - 1)];
+    }
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int j = j0 + wj * 64 + b * 32 + jl;
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = i0 + wi * 64 + a * 32 + (r & 3) + 8 * (r >> 2) + 4 * h2;
-                if (i < p.N && j < p.K) {
-                    float *to = out + (long)i * p.K + j;
-                    *to = p.accumulate ? *to + acc[a][b][r] : acc[a][b][r];
-                }
-            }
-        }
+            for (int r = 0; r < 16; ++r)
+                if (row_of(a, r) < p.N && col_of(b) < p.K) out[(long)row_of(a, r) * p.K + col_of(b)] = acc[a][b][r];
 }
 
 // ------------------------------------------------------------------------------------------
