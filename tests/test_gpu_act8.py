@@ -337,3 +337,19 @@ def test_weight_gradient_counts_the_last_rows_once(M, N, K):
     assert bool((ops.gemm_tn_act8(dy, codes, scales) == want).all())
     out = torch.full((N, K), 5.0, device=DEV)
     assert bool((ops.gemm_tn_act8(dy, codes, scales, out=out) == want + 5.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("M,E", [(1, 1), (5, 33), (7, 100), (131, 768), (300, 96), (9, 4104), (2000, 2048)])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("again", [False, True])
+def test_gradient_in_place_of_the_one_it_comes_from(M, E, dt, again):
+    """tc_dgelu_act8: du may be dy."""
+    lib, gen = _lib.load(), torch.Generator().manual_seed(M + E)
+    u, dy = torch.randn(M, E, generator=gen).to(dt).to(DEV), torch.randn(M, E, generator=gen).to(dt).to(DEV)
+    codes, scales = ops.act8_pack(u)
+    want, want_act = ops.dgelu_act8(dy, codes, scales, want_act=True)
+    act = torch.empty_like(dy)
+    assert lib.tc_dgelu_act8(int(dt == torch.bfloat16), dy.data_ptr(), E, codes.data_ptr(), scales.data_ptr(), dy.data_ptr(),
+                             act.data_ptr() if again else None, M, E, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(dy, want) and (not again or torch.equal(act, want_act))
