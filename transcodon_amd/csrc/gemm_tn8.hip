@@ -457,10 +457,13 @@ struct Tn8Plan {
     int splits;              // row splits, and parts of the sum
 };
 constexpr int kManySlabs = 16;
-constexpr long kPartBytes = 128L << 20;      // what the parts of a sum may always take; else a quarter of the operands' bytes
+// What the parts of a sum may take: this, or a quarter of the operands' bytes.  More of them gain little where products are that
+// large (231953 x 13736 x 12176: 7 parts, 4.7 GB, 65.7 ms; 3 parts, 2.0 GB, 66.9 ms; 20003 x 16384 x 4096: 2 parts 2.35 ms, 1 part 2.25).
+constexpr long kPartBytes = 128L << 20;
 // Which kernel and how many row splits: the least estimated time over both kernels and up to 256 splits, in nanoseconds.
 // A stage takes a large tile 1.9 us on a full chip (220 us at 65536 x 2304 x 768: 114 stages), a small one 1 us while
-// there is one workgroup per CU and 0.6 us more for each further one; a part of the sum costs its slab written and read at
+// there is one workgroup per CU and 0.6 us more for each further one (kernel trace, 768 x 768 on 36 CUs: 5.8 us for 64 rows, 0.8 us
+// for each further 64; the 2 us taken here for start and end are 5, but for every number of splits alike); a part of the sum costs its slab written and read at
 // 6.5 TB/s, and more than one the summing launch.
 Tn8Plan tn8_plan(long M, long ld_dy, int N, int K) {
     Tn8Plan best{};
