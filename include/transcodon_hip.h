@@ -766,7 +766,7 @@ int tc_dgelu_act8(int dtype, const void *dy, long ld_dy, const void *codes, cons
 /*
  * Weight gradient of a linear layer whose input is kept in 8 bits: dW[N,K] (+)= sum over m of dy[m,n] * v[m,k], f32, on the
  * matrix cores; v enters exactly, but below the smallest normal number (2^-126) it or its products may count as zero.  dy [M,N] bf16 with row stride ld_dy, codes [M,K], scales [M, ceil(K/32)] dense; N and
- * ld_dy multiples of 8, K of 16; 16-byte aligned.  The sum has a fixed order.  The workspace stays below the larger of 128 MiB and
+ * ld_dy multiples of 8, K of 16; 16-byte aligned.  The sum has a fixed order.  The workspace is at most the larger of 128 MiB and
  * a quarter of the bytes of dy and codes.
  */
 size_t tc_gemm_tn_act8_workspace_bytes(long M, long ld_dy, int N, int K);            /* 0: unsupported shape */
